@@ -189,6 +189,8 @@ int ensure_init() {
         k = norm_act_kernels(&n); add_kernels(k, n);
         k = nvfp4_gemm_kernels(&n); add_kernels(k, n);
         k = moe_kernels(&n); add_kernels(k, n);
+        k = moe_route_kernels(&n); add_kernels(k, n);
+        k = linear_kernels(&n); add_kernels(k, n);
     }
     e.ready = true;
     return 0;
@@ -209,6 +211,8 @@ void ensure_table() {
     k = norm_act_kernels(&n); add_kernels(k, n);
     k = nvfp4_gemm_kernels(&n); add_kernels(k, n);
     k = moe_kernels(&n); add_kernels(k, n);
+    k = moe_route_kernels(&n); add_kernels(k, n);
+    k = linear_kernels(&n); add_kernels(k, n);
 }
 
 // The tensor maps of a layer table whose record is dropped: captured graphs may still hold kernel nodes that point at

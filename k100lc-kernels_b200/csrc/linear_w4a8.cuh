@@ -1,0 +1,121 @@
+// What the kernels of the W4A8 product with an epilogue share: the arguments, the walk over the buckets of a plan, and
+// the epilogue.
+#pragma once
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace fm {
+namespace linear {
+
+constexpr int kMaxExperts = 1024;
+
+struct Params {
+    const uint8_t* wq;         // [n_exp][N or 2N][K/2]
+    const __half* ws;          // [n_exp][N or 2N][K/128]
+    const int8_t *ae, *ao;     // [xrows][K/2]
+    const float* asc;          // [xrows][K/128]
+    const int* asu;            // [xrows][K/128]
+    const float* bias;         // [n_exp][N or 2N] or nullptr
+    const float* residual;     // rows of ldr values or nullptr
+    float* y;                  // rows of ldy values
+    const int* bucket_rows;    // [m] or nullptr: slot s takes row s of x
+    const int* offsets;        // [n_exp + 1], or nullptr: one bucket of m rows
+    long long ldy, ldr;
+    int n_exp, m, xrows, N, K, act;
+    bool gated;
+};
+
+__device__ __forceinline__ float activate(int act, float v) {
+    switch (act) {
+        case 1: return v < 0.f ? 0.f : v;                               // (NaN stays NaN)
+        case 2: return __fdiv_rn(v, 1.f + expf(-v));
+        case 3: return 0.5f * v * erfcf(v * -0.70710678f);                // 1 + erf(t) = erfc(-t): no cancellation for v < 0
+        case 4: return __fdiv_rn(v, 1.f + expf(-1.5957691f * (v + 0.044715f * v * v * v)));   // 1 + tanh(t) = 2 / (1 + exp(-2t))
+        default: return v;
+    }
+}
+__device__ __forceinline__ void finish(const Params& p, const float* bias, size_t m, int n, float v) {
+    if (bias) v += bias[n];
+    v = activate(p.act, v);
+    if (p.residual) v += p.residual[m * p.ldr + n];
+    p.y[m * p.ldy + n] = v;
+}
+__device__ __forceinline__ void finish_gated(const Params& p, const float* bias, size_t m, int n, float gate, float up) {
+    if (bias) {
+        gate += bias[n];
+        up += bias[p.N + n];
+    }
+    float v = activate(p.act, gate) * up;
+    if (p.residual) v += p.residual[m * p.ldr + n];
+    p.y[m * p.ldy + n] = v;
+}
+
+// A unit is one tile of weight rows times one chunk of a bucket's rows; units of a chunk differ in the tile last.
+struct Unit { int expert, tile, first, count, pad; };
+struct Buckets { int part[33]; };
+
+// bounds of bucket e, held to [0, m]: a damaged plan cannot lead out of the output
+__device__ __forceinline__ int bound(const Params& p, int e) { return min(max(p.offsets[e], 0), p.m); }
+
+// Number of units; ends[e] becomes the number of units of the experts up to e.  All threads of the CTA call it.
+__device__ __forceinline__ int count_units(const Params& p, int cols, int tiles, int* ends, Buckets* bk) {
+    if (!p.offsets) return (p.m + cols - 1) / cols * tiles;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    int carry = 0;
+    for (int e0 = 0; e0 < p.n_exp; e0 += blockDim.x) {
+        const int e = e0 + (int)threadIdx.x;
+        int v = 0;
+        if (e < p.n_exp) v = (max(bound(p, e + 1) - bound(p, e), 0) + cols - 1) / cols * tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += t;
+        }
+        __syncthreads();
+        if (lane == 31) bk->part[warp] = v;
+        __syncthreads();
+        int all = 0;
+        for (int k = 0; k < warps; k++) {
+            if (k < warp) v += bk->part[k];
+            all += bk->part[k];
+        }
+        if (e < p.n_exp) ends[e] = carry + v;
+        carry += all;
+    }
+    __syncthreads();
+    return carry;
+}
+
+__device__ __forceinline__ Unit find_unit(const Params& p, int u, int cols, int tiles, const int* ends) {
+    Unit r;
+    int lo = 0, begin = 0, end = p.m;
+    if (p.offsets) {
+        int hi = p.n_exp - 1;                                         // first expert whose units end behind u
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (ends[mid] > u) hi = mid;
+            else lo = mid + 1;
+        }
+        if (lo) u -= ends[lo - 1];
+        begin = bound(p, lo);
+        end = bound(p, lo + 1);
+    }
+    const int chunks = (end - begin + cols - 1) / cols;
+    r.expert = lo;
+    r.tile = u / chunks;
+    r.first = begin + (u - r.tile * chunks) * cols;
+    r.count = min(cols, end - r.first);
+    r.pad = 0;
+    return r;
+}
+
+// row of x that column c of the unit takes, or -1
+__device__ __forceinline__ long long x_row(const Params& p, const Unit& u, int c) {
+    if (c >= u.count) return -1;
+    if (!p.bucket_rows) return u.first + c;
+    const int r = p.bucket_rows[u.first + c];
+    return r >= 0 && r < p.xrows ? r : -1;
+}
+
+}  // namespace linear
+}  // namespace fm

@@ -6,6 +6,7 @@ from .catalog import info, kernels
 from .model import (Attention, DotLinear, F32Linear, FlashAttention, Int4Linear, KVCache, MLP,
                     MoECombine, MoEExperts, NVFP4Linear, RMSNorm, RoPE, RT4Linear, Sampler, SwiGLU,
                     TransformerLayer, Workspace, div_magic, run_sequence)
+from .moe import ExpertLinear, FusedLinear, MoEMLP, MoEPlan, MoERouter
 from .quant import (ct_int4_to_rt4, ct_int4_to_twos_complement, dequant_int4_group128,
                     int4_scale_group_first_f32, pack_int4_group128)
 from .rt4 import RT4File, RT4Tensor, W4Runner
@@ -14,7 +15,8 @@ from .runtime import LaunchPlan, Runtime
 __all__ = [
     "Runtime", "LaunchPlan", "kernels", "info", "RT4File", "RT4Tensor", "W4Runner", "Workspace",
     "DotLinear", "F32Linear", "RT4Linear", "Int4Linear", "NVFP4Linear", "Attention", "FlashAttention",
-    "TransformerLayer", "RMSNorm", "SwiGLU", "MLP", "MoECombine", "MoEExperts", "RoPE", "KVCache",
+    "TransformerLayer", "RMSNorm", "SwiGLU", "MLP", "MoECombine", "MoEExperts", "MoERouter", "MoEPlan",
+    "MoEMLP", "FusedLinear", "ExpertLinear", "RoPE", "KVCache",
     "Sampler", "div_magic", "run_sequence", "pack_int4_group128", "dequant_int4_group128",
     "ct_int4_to_rt4", "ct_int4_to_twos_complement", "int4_scale_group_first_f32",
 ]

@@ -1,0 +1,150 @@
+"""GPU tier: moe_route_k and moe_plan_k against the plain 64-bit forms — whole numbers equal, weights within fp32's
+error — and the calls that they refuse."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import moe_plain as P
+from gpu_util import Bufs
+from k100lc_kernels import MoERouter, Workspace
+
+pytestmark = pytest.mark.gpu
+
+
+def _rounded(x, dtype):
+    """(bits for the device, the values they stand for)"""
+    if dtype == "f32":
+        return x.astype(np.float32), x.astype(np.float32)
+    if dtype == "f16":
+        return x.astype(np.float16), x.astype(np.float16).astype(np.float32)
+    bits = (x.astype(np.float32).view(np.uint32) >> 16).astype(np.uint16)
+    return bits, (bits.astype(np.uint32) << 16).view(np.float32)
+
+
+def _run(rt, x, dtype="f32", **kw):
+    rows, n_exp = x.shape
+    bits, values = _rounded(x, dtype)
+    topk = kw["topk"]
+    with Workspace(rt) as ws:
+        router = MoERouter(rt, n_exp, dtype=dtype, ws=ws, **kw)
+        plan = router.forward_device(ws.upload("x", bits) if rows else 0, rows, sync=True)
+        get = lambda p, n, t: rt.download(p, n, t)  # noqa: E731
+        got = dict(ids=get(plan.ids, rows * topk, np.int32).reshape(rows, topk), w=get(plan.weights, rows * topk, np.float32).reshape(rows, topk),
+                   bucket=get(plan.bucket_rows, rows * topk, np.int32), base=get(plan.base, rows * topk, np.int32).reshape(rows, topk),
+                   offsets=get(plan.offsets, n_exp + 1, np.int32))
+    return got, values
+
+
+def _check(got, values, **kw):
+    ids, w = P.route(values, **kw)
+    assert np.array_equal(got["ids"], ids)
+    assert np.all(np.abs(got["w"] - w) <= P.ROUTE_REL * np.abs(w) + 2.0 ** -126)
+    bucket, base, _w, offsets = P.plan(got["ids"], got["w"], values.shape[1])
+    assert np.array_equal(got["offsets"], offsets) and np.array_equal(got["base"], base)
+    assert np.array_equal(got["bucket"][: bucket.size], bucket)
+
+
+@pytest.mark.parametrize("rows,n_exp,topk", [(1, 1, 1), (1, 8, 2), (3, 33, 5), (7, 60, 4), (64, 128, 8), (5, 1024, 32), (257, 513, 3),
+                                             (1000, 256, 8), (4099, 64, 6)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_sizes(rt, rows, n_exp, topk, score, biased):
+    rng = np.random.default_rng(rows * 1000 + n_exp)
+    x = (rng.standard_normal((rows, n_exp)) * 2).astype(np.float32)
+    kw = dict(topk=topk, score=score, bias=(rng.standard_normal(n_exp) * 0.1).astype(np.float32) if biased else None)
+    got, values = _run(rt, x, **kw)
+    _check(got, values, **kw)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n_exp,n_group,topk_group,group_top", [(256, 8, 4, 2), (60, 4, 2, 1), (36, 12, 5, 2), (32, 32, 8, 2), (1024, 2, 1, 2), (40, 1, 1, 1)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_groups_and_types(rt, dtype, n_exp, n_group, topk_group, group_top, biased):
+    rng = np.random.default_rng(n_exp + n_group)
+    x = rng.standard_normal((301, n_exp)) * 1.5
+    kw = dict(topk=min(8, n_exp // n_group * topk_group), score="sigmoid", n_group=n_group, topk_group=topk_group, group_top=group_top,
+              bias=(rng.standard_normal(n_exp) * 0.05).astype(np.float32) if biased else None, scale=2.5)
+    got, values = _run(rt, x, dtype, **kw)
+    _check(got, values, **kw)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_route_masks_ties_and_infinities(rt, score, renorm):
+    inf, nan = np.inf, np.nan
+    x = np.zeros((9, 40), np.float32)
+    x[0] = -inf                                            # nothing to choose
+    x[1] = nan
+    x[2, 3:] = -inf                                        # three candidates for five choices
+    x[3] = np.finfo(np.float32).min                        # the type's lowest value is a number
+    x[4, 5], x[4, 6] = inf, inf
+    x[5, ::2] = -0.0                                       # -0 and +0 tie
+    x[6] = np.arange(40) % 7
+    x[7, 11] = nan
+    x[8, 39] = 30
+    if score == "sigmoid":
+        x[3] = -80
+    for bias in (None, np.zeros(40, np.float32), np.where(np.arange(40) == 0, -inf, 0).astype(np.float32)):
+        kw = dict(topk=5, score=score, renorm=renorm, bias=bias)
+        got, values = _run(rt, x, **kw)
+        _check(got, values, **kw)
+
+
+def test_route_resolves_keys_that_fp32_cannot(rt):
+    """Logits one step apart and large biases: many keys agree in 32 bits and differ in 64."""
+    rng = np.random.default_rng(5)
+    step = np.float32(1.0)
+    row = []
+    for _ in range(64):
+        row.append(step)
+        step = np.nextafter(step, np.float32(2))
+    x = np.stack([rng.permutation(np.array(row, np.float32)) for _ in range(200)])
+    for score in ("softmax", "sigmoid"):
+        for b in (np.zeros(64), np.full(64, 3.0), np.where(np.arange(64) < 32, 100.0, 100.0 + 2.0 ** -17)):
+            kw = dict(topk=8, score=score, bias=b.astype(np.float32))
+            got, values = _run(rt, x, **kw)
+            _check(got, values, **kw)
+            kw |= dict(n_group=8, topk_group=3, group_top=2)
+            got, values = _run(rt, x, **kw)
+            _check(got, values, **kw)
+
+
+def test_route_no_rows(rt):
+    got, _ = _run(rt, np.zeros((0, 8), np.float32), topk=2)
+    assert np.array_equal(got["offsets"], np.zeros(9, np.int32))
+
+
+@pytest.mark.parametrize("rows,n_exp,topk", [(1, 1, 1), (1, 1024, 32), (33, 5, 3), (2048, 8, 1), (2049, 8, 1), (5000, 300, 7), (40000, 64, 8)])
+def test_plan_of_given_pairs(rt, rows, n_exp, topk):
+    """Ids out of range, repeated experts and zero weights; slots behind the last bucket stay as they were."""
+    rng = np.random.default_rng(rows)
+    ids = rng.integers(-2, n_exp + 2, size=(rows, topk)).astype(np.int32)
+    w = rng.random((rows, topk)).astype(np.float32)
+    w[rng.random((rows, topk)) < 0.1] = 0
+    with Bufs(rt) as b:
+        pw, pr, pb, po = b.put(w), b.zeros(rows * topk, np.int32, -7), b.zeros(rows * topk, np.int32, -7), b.zeros(n_exp + 1, np.int32, -7)
+        rt.launch("moe_plan_k", 1, 1, [b.put(ids), pw, pr, pb, po, rows, n_exp, topk])
+        got = [b.get(pr, rows * topk, np.int32), b.get(pb, rows * topk, np.int32).reshape(rows, topk), b.get(pw, rows * topk).reshape(rows, topk),
+               b.get(po, n_exp + 1, np.int32)]
+    bucket, base, wz, offsets = P.plan(ids, w, n_exp)
+    assert np.array_equal(got[0][: bucket.size], bucket) and np.all(got[0][bucket.size:] == -7)
+    assert np.array_equal(got[1], base) and np.array_equal(got[2], wz) and np.array_equal(got[3], offsets)
+
+
+def test_route_and_plan_refuse(rt):
+    with Bufs(rt) as b:
+        x, ids, w = b.zeros(64), b.zeros(16, np.int32), b.zeros(16)
+        ok = [x, 0, ids, w, 8, 8, 2, 1, 1, 1, 0, 1, 1.0, 0]
+        rt.launch("moe_route_k", 1, 1, ok)
+        for at, bad in ((4, -1), (4, 9), (5, 0), (5, 1025), (5, 9), (6, 0), (6, 9), (7, 3), (8, 2), (9, 0), (10, 2), (11, 2), (13, 3), (0, x + 2),
+                        (0, x + 4), (1, x + 240), (2, ids + 4), (3, w + 4), (0, 0)):
+            with pytest.raises(RuntimeError, match="rejected"):
+                rt.launch("moe_route_k", 1, 1, ok[:at] + [bad] + ok[at + 1:])
+        bucket, base, off = b.zeros(16, np.int32), b.zeros(16, np.int32), b.zeros(9, np.int32)
+        ok = [ids, w, bucket, base, off, 8, 8, 2]
+        rt.launch("moe_plan_k", 1, 1, ok)
+        for at, bad in ((5, -1), (5, 9), (6, 0), (6, 9), (6, 1025), (7, 0), (7, 33), (0, ids + 4), (1, 0), (2, bucket + 4), (3, base + 2), (4, off + 4)):
+            with pytest.raises(RuntimeError, match="rejected"):
+                rt.launch("moe_plan_k", 1, 1, ok[:at] + [bad] + ok[at + 1:])
+        rt.sync()
