@@ -265,10 +265,24 @@ def _plain_experts(s):
 
 
 # ------------------------------------------------------------------------------------------- the package's calls
-class _Memory:
-    """Names memory of the engine to torch."""
+class _Buffers:
+    """Device buffers of one state, freed when neither the state nor one of its outputs is in use any more."""
 
-    def __init__(self, ptr, shape, typestr):
+    def __init__(self, workspace):
+        self.workspace = workspace
+
+    def view(self, ptr, shape, typestr):
+        return torch.as_tensor(_Memory(self, ptr, shape, typestr), device="cuda")
+
+    def __del__(self):
+        self.workspace.free()
+
+
+class _Memory:
+    """Names memory of the engine to torch; a tensor made from it keeps the buffers."""
+
+    def __init__(self, owner, ptr, shape, typestr):
+        self.owner = owner
         self.__cuda_array_interface__ = {"data": (ptr, False), "shape": tuple(shape), "typestr": typestr, "version": 3}
 
 
@@ -284,13 +298,14 @@ class _Engine:
         if _Engine.runtime is None:
             _Engine.runtime = kk.Runtime()
         rt, case = _Engine.runtime, s["case"]
-        self.ws = ws = kk.Workspace(rt)
+        ws = kk.Workspace(rt)
+        self.buffers, self.views = _Buffers(ws), {}
 
         def put(name, t):
             if t is None:
                 return None
             p = ws.buffer(name, t.numel() * t.element_size())
-            self.view(p, (t.numel() * t.element_size(),), "|u1").copy_(t.contiguous().view(-1).view(torch.uint8))
+            self.buffers.view(p, (t.numel() * t.element_size(),), "|u1").copy_(t.contiguous().view(-1).view(torch.uint8))
             return p
 
         rows = case["rows"]
@@ -300,6 +315,7 @@ class _Engine:
                                    topk_group=case["kept"], group_top=case["group_top"], scale=case["scale"],
                                    dtype=case["dtype"], ws=ws)
             self.logits = put("logits", s["logits"])
+            torch.cuda.synchronize()                                  # the engine has a stream of its own
             return
         wq, scales, bias = put("wq", s["wq"]), put("ws", s["ws"]), put("bias", s["bias"])
         self.codes = tuple(put(n, s["codes"][n]) for n in ("ae", "ao", "asc", "asu"))
@@ -313,25 +329,19 @@ class _Engine:
                                    **{n: put("plan." + n, t) for n, t in s["plan"].items()})
             rows = rows * case["topk"]
         self.out = ws.buffer("out", rows * case["n"] * 4)
-        self.result = self.view(self.out, (rows, case["n"]), "<f4")
+        self.result = self.buffers.view(self.out, (rows, case["n"]), "<f4")
         torch.cuda.synchronize()
-
-    @staticmethod
-    def view(ptr, shape, typestr):
-        return torch.as_tensor(_Memory(ptr, shape, typestr), device="cuda")
-
-    def __del__(self):
-        if getattr(self, "ws", None) is not None:
-            self.ws.free()
 
     def run(self, case):
         if case["op"] == "route":
             plan = self.op.forward_device(self.logits, case["rows"])
-            pairs = (case["rows"], case["topk"])
-            return {"ids": self.view(plan.ids, pairs, "<i4"), "weights": self.view(plan.weights, pairs, "<f4"),
-                    "bucket_rows": self.view(plan.bucket_rows, (pairs[0] * pairs[1],), "<i4"),
-                    "base": self.view(plan.base, pairs, "<i4"),
-                    "offsets": self.view(plan.offsets, (case["experts"] + 1,), "<i4")}
+            if not self.views:                                        # the router's buffers, named once
+                pairs, view = (case["rows"], case["topk"]), self.buffers.view
+                self.views = {"ids": view(plan.ids, pairs, "<i4"), "weights": view(plan.weights, pairs, "<f4"),
+                              "bucket_rows": view(plan.bucket_rows, (pairs[0] * pairs[1],), "<i4"),
+                              "base": view(plan.base, pairs, "<i4"),
+                              "offsets": view(plan.offsets, (case["experts"] + 1,), "<i4")}
+            return self.views
         if case["op"] == "linear":
             self.op.forward_codes_device(self.codes, case["rows"], residual_dev=self.residual, out_dev=self.out)
         else:
