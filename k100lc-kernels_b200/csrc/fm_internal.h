@@ -61,6 +61,8 @@ bool encode_chunk_maps(void* wmap128, void* smap128, const void* wbase, const vo
 const void* stream_table_maps(const void* table, int nlayers, int rows, int K);
 // one such map (gemm_w4.cu holds the encoder): false when the driver refuses it
 bool encode_bytes_rows_map(void* map128, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_bytes);
+// the same with a box of box_rows rows
+bool encode_bytes_box_map(void* map128, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_bytes, uint32_t box_rows);
 
 // true when [ptr, ptr+bytes) lies inside the local window that fm_stream_peers validated for the offset array
 // `peer_delta` (so every receiver has the same bytes at the same offset), or checks are off
@@ -101,6 +103,7 @@ namespace stream { struct StreamParams; }
 int nvfp4_tc_stream(const char* kn, const LaunchCtx& c, const stream::StreamParams& sp, float gscale, bool dump);
 int stream_read_status(cudaStream_t stream);   // 0, or the code of the first bounded wait that ran out in such a launch
 
+int linear_read_status();                    // the same for the tiles of linear_w4a8_tc.cu (the stream is drained already)
 int gemm_read_status(cudaStream_t stream);   // 0, or the code of the first bounded wait that ran out
 
 // argv decoding ------------------------------------------------------------

@@ -109,17 +109,6 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* b, uint32_t parity, Cont
     return false;
 }
 
-// two fp32 lanes per instruction (sm_100 packed fp32): per lane identical to fmul / fmaf
-__device__ __forceinline__ void mul2(float& d0, float& d1, float a, float b0, float b1) {
-    asm("{\n.reg .b64 ra, rb, rd;\nmov.b64 ra, {%2,%2};\nmov.b64 rb, {%3,%4};\nmul.rn.f32x2 rd, ra, rb;\nmov.b64 {%0,%1}, rd;\n}"
-        : "=f"(d0), "=f"(d1) : "f"(a), "f"(b0), "f"(b1));
-}
-__device__ __forceinline__ void fma2(float& c0, float& c1, float a0, float a1, float b0, float b1) {
-    asm("{\n.reg .b64 ra, rb, rc;\nmov.b64 ra, {%2,%3};\nmov.b64 rb, {%4,%5};\nmov.b64 rc, {%0,%1};\n"
-        "fma.rn.f32x2 rc, ra, rb, rc;\nmov.b64 {%0,%1}, rc;\n}"
-        : "+f"(c0), "+f"(c1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
-
 // Weights: K-major, no swizzle: start address, LBO (next core matrix in K), SBO (next 8-row group)
 __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr) {
     uint64_t d = 0;
@@ -521,14 +510,14 @@ EncodeTiledFn tensor_map_encoder() {
     }();
     return fn;
 }
-// bytes [rows][row_bytes], row-major and dense; box = box_bytes x 128 rows
+// bytes [rows][row_bytes], row-major and dense; box = box_bytes x box_rows
 bool make_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_bytes, CUtensorMapSwizzle sw,
-              CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_128B) {
+              CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_128B, uint32_t box_rows = 128) {
     EncodeTiledFn enc = tensor_map_encoder();
     if (!enc) return false;
     const cuuint64_t dims[2] = {row_bytes, rows};
     const cuuint64_t strides[1] = {row_bytes};
-    const cuuint32_t box[2] = {box_bytes, 128};
+    const cuuint32_t box[2] = {box_bytes, box_rows};
     const cuuint32_t estr[2] = {1, 1};
     return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, sw, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -711,6 +700,10 @@ bool encode_chunk_maps(void* wmap128, void* smap128, const void* wbase, const vo
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+bool encode_bytes_box_map(void* map128, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_bytes, uint32_t box_rows) {
+    return make_map(static_cast<CUtensorMap*>(map128), base, rows, row_bytes, box_bytes,
+                    box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, box_rows);
+}
 bool encode_bytes_rows_map(void* map128, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_bytes) {
     // (256-byte L2 promotion: the next stage's 128 bytes of a row come along; 1 % over 128 bytes or none)
     return make_map(static_cast<CUtensorMap*>(map128), base, rows, row_bytes, box_bytes,
@@ -722,7 +715,8 @@ int gemm_read_status(cudaStream_t stream) {
     if (cudaStreamSynchronize(stream) != cudaSuccess) return -1;
     if (cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(int)) != cudaSuccess) return -1;
     cudaMemcpyToSymbol(g_gemm_status, &zero, sizeof(int));
-    return v;
+    const int w = linear_read_status();
+    return v ? v : w;
 }
 
 }  // namespace fm

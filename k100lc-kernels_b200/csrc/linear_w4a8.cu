@@ -159,6 +159,9 @@ cudaError_t run_rows(const LaunchCtx& c, const Params& p) {
 }
 
 int run(const char* kn, const LaunchCtx& c, const Params& p) {
+    // rows per bucket, were all experts equally popular
+    const int per = p.offsets ? p.m / (p.n_exp < p.m ? p.n_exp : p.m) : p.m;
+    if (per >= 16) return run_tiles(kn, c, p);
     const cudaError_t e = p.m <= 8 || p.offsets ? run_rows<1>(c, p) : run_rows<2>(c, p);
     return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
 }

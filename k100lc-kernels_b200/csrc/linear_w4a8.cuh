@@ -4,6 +4,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "fm_internal.h"
+
 namespace fm {
 namespace linear {
 
@@ -116,6 +118,9 @@ __device__ __forceinline__ long long x_row(const Params& p, const Unit& u, int c
     const int r = p.bucket_rows[u.first + c];
     return r >= 0 && r < p.xrows ? r : -1;
 }
+
+// the tensor-core tiles (linear_w4a8_tc.cu); arguments checked
+int run_tiles(const char* kn, const LaunchCtx& c, const Params& p);
 
 }  // namespace linear
 }  // namespace fm

@@ -1,0 +1,427 @@
+// The W4A8 product with an epilogue on the fifth-generation tensor cores, for buckets of many rows (the entries and the
+// arithmetic are those of linear_w4a8.cu).
+//
+// D^T[weight row][row of x] = W . x^T: 128 weight rows (gated: 64 gate rows and the 64 up rows beside them) are the 128
+// lanes of an accumulator, up to 128 rows of a bucket its columns, so that a short bucket costs a narrow MMA and not a
+// padded tile.  The product of a 128-group is one exact integer, formed as a float: int4 weights and int8 codes are
+// exact in f16, a product is below 2^10, a sum of 128 below 2^17, so tcgen05.mma.kind::f16 with fp32 accumulators
+// returns float(I) and the epilogue needs no conversion (with kind::i8 the conversions, 16 a clock per SM, take four
+// times as long as the MMAs).
+//
+// Roles of the 24 warps of the persistent CTA, joined by mbarriers (every wait is bounded):
+//   * one lane copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring;
+//   * eight warps expand them: a thread owns a weight row, reads its 64 bytes, turns nibbles into f16 pairs with four
+//     logic and four arithmetic instructions a word, and writes them to tensor memory, from where the MMA takes its A
+//     operand: no shared-memory traffic for the wide operand, which would otherwise bound the tile (128 bytes a clock);
+//   * four warps fetch the rows of x (f16, expanded once per call by a small kernel in front, k in the order of the
+//     nibble pairs) with 16-byte cp.async, gathering them by the plan, into the 128-byte-swizzled layout of B;
+//   * two threads issue the MMAs of the even and the odd groups into two accumulators;
+//   * eight warps drain the accumulators: C[m, n] = fmaf(float(I), ws * asc, C) in registers, then the epilogue.
+#include <cuda.h>
+
+#include "device_utils.cuh"
+#include "fm_internal.h"
+#include "linear_w4a8.cuh"
+#include "tc_utils.cuh"
+
+namespace fm {
+namespace linear {
+namespace {
+using namespace tc;
+
+constexpr int kCols = 128;                          // rows of x per tile
+constexpr int RING = 4;                             // stages of A (tensor memory), B (shared memory) and "step done" barriers
+constexpr int BP = 6;                               // stages of packed weights
+constexpr int SLOTS = 8;                            // stages of activation scales (reuse distance: see the loaders)
+constexpr int kLag = 2;                             // steps between issuing a row fetch and publishing it
+constexpr int B_BYTES = kCols * 256, BP_BYTES = 128 * 64;
+constexpr int MMA_WARP = 1, LOAD_WARP0 = 4, EXP_WARP0 = 8, EPI_WARP0 = 16, kThreads = 24 * 32;
+// 768 threads start with 80 registers each (61 440 of the file); the shares below add up to the same
+constexpr int kRegsIssue = 32, kRegsLoad = 64, kRegsExpand = 72, kRegsEpilogue = 120;
+static_assert(kRegsIssue + kRegsLoad + 2 * kRegsExpand + 2 * kRegsEpilogue == 480, "register shares of the six warpgroups");
+static_assert(SLOTS >= RING + 2, "a scale slot is rewritten RING steps ahead of the MMAs, which are 2 ahead of the epilogue");
+constexpr int kSpin = 1 << 17;
+constexpr uint32_t kTmemCols = 512, kTmemA = 256;   // accumulators: columns 0..255; A: 4 x 64 columns
+
+struct __align__(16) Control {
+    uint64_t bp_full[BP], bp_free[BP];
+    uint64_t a_full[RING], b_full[RING], done[RING];
+    uint64_t acc_free[2], drain[2];
+    uint32_t tmem_base;
+    volatile int abort;
+};
+
+__device__ int g_status;                            // 0, or the code 21.. of the first bounded wait that ran out
+
+__device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity, Control* ctl, int code) {
+    for (int i = 0; i < kSpin; i++) {
+        if (mbar_try_wait(b, parity)) return true;
+        if ((i & 63) == 63 && ctl->abort) return false;
+    }
+    ctl->abort = 1;
+    atomicCAS(&g_status, 0, code);
+    return false;
+}
+
+// the same by all lanes of a warp, which leave it with one answer (their next instructions are warp-wide)
+__device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, Control* ctl, int code) {
+    return __all_sync(0xffffffffu, wait(b, parity, ctl, code));
+}
+
+// kind::f16: f32 accumulator, f16 operands, both K-major, M = 128
+__device__ __forceinline__ uint32_t instr_desc(int n) { return 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24; }
+
+// Eight two's-complement nibbles of a word -> four f16 pairs (k0,k4) (k1,k5) (k2,k6) (k3,k7), exact: 0x6400 is 1024 with
+// steps of 1, so nibble ^ 8 in the low bits is 1024 + u, and in the next four bits 1024 + 16 u.
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ void expand_word(uint32_t w, uint32_t* o) {
+    const uint32_t v = w >> 8;
+    o[0] = sub_f16x2((w & 0x000F000Fu) ^ 0x64086408u, 0x64086408u);                          // - 1032
+    o[1] = fma_f16x2((w & 0x00F000F0u) ^ 0x64806480u, 0x2C002C00u, 0xD480D480u);             // / 16 - 72
+    o[2] = sub_f16x2((v & 0x000F000Fu) ^ 0x64086408u, 0x64086408u);
+    o[3] = fma_f16x2((v & 0x00F000F0u) ^ 0x64806480u, 0x2C002C00u, 0xD480D480u);
+}
+
+// codes [rows][K/2] even and odd -> f16 [rows][K] in the pair order above
+__global__ void __launch_bounds__(256)
+expand_codes_kernel(const uint2* __restrict__ ae, const uint2* __restrict__ ao, uint4* __restrict__ out, size_t n) {
+    pdl_wait();
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
+        const uint2 e = ae[i], o = ao[i];                            // 16 k
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t a = h ? e.y : e.x, b = h ? o.y : o.x;
+            auto pair = [](uint32_t w, int j) {                      // bytes j and j + 2
+                const __half2 v = __floats2half2_rn((float)(int8_t)(w >> (8 * j)), (float)(int8_t)(w >> (8 * j + 16)));
+                return *reinterpret_cast<const uint32_t*>(&v);
+            };
+            out[2 * i + h] = make_uint4(pair(a, 0), pair(b, 0), pair(a, 1), pair(b, 1));
+        }
+    }
+    pdl_launch_dependents();
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
+}
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <bool GATED>
+__global__ void __launch_bounds__(kThreads, 1)
+tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __half* __restrict__ xh) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* bring = smem;                                           // RING x [2 halves of 64 k][128 rows][128 bytes]
+    uint8_t* wring = bring + RING * B_BYTES;                         // BP x [128 rows][64 bytes]
+    float* sring = reinterpret_cast<float*>(wring + BP * BP_BYTES);  // SLOTS x [128]
+    float* xch = sring + SLOTS * kCols;                              // [128 columns][64 rows]: up values on their way to the gate lanes
+    Control* ctl = reinterpret_cast<Control*>(xch + (GATED ? kCols * 64 : 0));
+    int* ends = reinterpret_cast<int*>(ctl + 1);                     // [n_exp]
+    __shared__ Buckets bk;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int ROWS = GATED ? 64 : 128;
+    const int G = p.K / 128, tiles = (p.N + ROWS - 1) / ROWS;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < BP; i++) {
+            mbar_init(&ctl->bp_full[i], 1);
+            mbar_init(&ctl->bp_free[i], 4);
+        }
+        for (int i = 0; i < RING; i++) {
+            mbar_init(&ctl->a_full[i], 4);
+            mbar_init(&ctl->b_full[i], 4);
+            mbar_init(&ctl->done[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&ctl->acc_free[i], 8);
+            mbar_init(&ctl->drain[i], 1);
+        }
+        ctl->abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == MMA_WARP) tmem_alloc(&ctl->tmem_base, kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+    pdl_wait();
+    const int total = count_units(p, kCols, tiles, ends, &bk);
+
+    if (warp < LOAD_WARP0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+        if (warp == 0 && lane == 0) {
+            // ================================================================ packed weights
+            int it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+                const Unit un = find_unit(p, u, kCols, tiles, ends);
+                const int y0 = un.expert * (GATED ? 2 * p.N : p.N) + un.tile * ROWS, y1 = y0 + (GATED ? p.N : 64);
+                for (int g = 0; g < G; g++, it++) {
+                    const int s = it % BP;
+                    if (it >= BP && !(ok = wait(&ctl->bp_free[s], ((it / BP) & 1) ^ 1, ctl, 21))) break;
+                    mbar_expect_tx(&ctl->bp_full[s], BP_BYTES);
+                    tma_2d(wring + s * BP_BYTES, &map, g * 64, y0, &ctl->bp_full[s]);
+                    tma_2d(wring + s * BP_BYTES + BP_BYTES / 2, &map, g * 64, y1, &ctl->bp_full[s]);
+                }
+            }
+            if (ctl->abort)                                          // copies in flight land before the memory is given up
+                for (int j = it > BP ? it - BP : 0; j < it; j++)
+                    for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->bp_full[j % BP], (j / BP) & 1); i++) {}
+        } else if ((warp == MMA_WARP || warp == MMA_WARP + 1) && lane == 0) {
+            // ================================================================ MMA issuers: even and odd steps
+            const int par = warp - MMA_WARP;
+            const uint64_t bdesc0 = smem_desc_sw128(smem_u32(bring));
+            int it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+                const Unit un = find_unit(p, u, kCols, tiles, ends);
+                const uint32_t idesc = instr_desc((un.count + 15) & ~15);
+                for (int g = 0; g < G; g++, it++) {
+                    if ((it & 1) != par) continue;
+                    const int s = it % RING;
+                    const uint32_t ph = (it / RING) & 1;
+                    if (it >= 2 && !(ok = wait(&ctl->acc_free[par], ((it >> 1) & 1) ^ 1, ctl, 22))) break;
+                    if (!(ok = wait(&ctl->a_full[s], ph, ctl, 23))) break;
+                    if (!(ok = wait(&ctl->b_full[s], ph, ctl, 24))) break;
+                    tc_fence_after();
+                    const uint64_t bd = bdesc0 + (uint64_t)(s * (B_BYTES >> 4));
+                    const uint32_t d = tmem + par * kCols, a = tmem + kTmemA + s * 64;
+#pragma unroll
+                    for (int j = 0; j < 8; j++)                      // 16 k each: 8 columns of A, 32 bytes of B
+                        tc_mma_f16_ts(d, a + j * 8, bd + (j >> 2) * (kCols * 128 >> 4) + (j & 3) * 2, idesc, j > 0);
+                    tc_commit(&ctl->done[s]);
+                }
+            }
+            // nothing this thread issued may still run when tensor memory is released
+            tc_commit(&ctl->drain[par]);
+            for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->drain[par], 0); i++) {}
+        }
+    } else if (warp < EXP_WARP0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
+        // ==================================================================== rows of x and their scales
+        // Thread i fetches chunk i % 16 (16 bytes) of the rows i / 16, i / 16 + 8, ..., and the scale of row i.  Slot
+        // it % SLOTS of the scales was last read by the epilogue of step it - SLOTS: stage it % RING is free when the MMAs of step
+        // it - RING have run, which were issued after the accumulator of step it - RING - 2 had been drained.
+        const int i = threadIdx.x - LOAD_WARP0 * 32, c = i & 15, r0 = i >> 4;
+        const uint32_t dst0 = smem_u32(bring) + (c >> 3) * (kCols * 128) + r0 * 128 + (((c & 7) ^ r0) << 4);
+        const uint32_t sdst0 = smem_u32(sring) + i * 4;
+        int it = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+            const Unit un = find_unit(p, u, kCols, tiles, ends);
+            const int n16 = (un.count + 15) & ~15;
+            uint32_t off[16];                                        // rows in units of 16 bytes; ~0: zeros
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const long long r = r0 + 8 * j < n16 ? x_row(p, un, r0 + 8 * j) : -1;
+                off[j] = r < 0 ? ~0u : (uint32_t)(r * (p.K / 8));
+            }
+            const long long sr = x_row(p, un, i);
+            const float* sc = p.asc + (sr < 0 ? 0 : (size_t)sr * G);
+            const uint4* src = reinterpret_cast<const uint4*>(xh) + c;
+            for (int g = 0; g < G; g++, it++, src += 16) {
+                const int s = it % RING;
+                if (it >= RING && !(ok = wait_warp(&ctl->done[s], ((it / RING) & 1) ^ 1, ctl, 25))) break;
+                const uint32_t dst = dst0 + s * B_BYTES;
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (8 * j < n16) cp_async16(dst + j * 1024, off[j] == ~0u ? src : src + off[j], off[j] != ~0u);
+                cp_async4(sdst0 + (it % SLOTS) * (kCols * 4), sc + g, sr >= 0);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (it >= kLag) {
+                    cp_async_wait<kLag>();
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl->b_full[(it - kLag) % RING]);
+                }
+            }
+        }
+        cp_async_wait<0>();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (ok && lane == 0)
+            for (int j = it > kLag ? it - kLag : 0; j < it; j++) mbar_arrive(&ctl->b_full[j % RING]);
+    } else if (warp < EPI_WARP0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsExpand));
+        // ==================================================================== expansion of the weights
+        const int set = (warp - EXP_WARP0) >> 2, q = warp & 3, row = q * 32 + lane;
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        int it = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+            for (int g = 0; g < G; g++, it++) {
+                if ((it & 1) != set) continue;
+                const int sp = it % BP, s = it % RING;
+                if (!(ok = wait_warp(&ctl->bp_full[sp], (it / BP) & 1, ctl, 26))) break;
+                uint4 w[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++)                          // 64-byte swizzle: chunk ^= (row / 2) % 4
+                    w[j] = *reinterpret_cast<const uint4*>(wring + sp * BP_BYTES + row * 64 + ((j ^ ((row >> 1) & 3)) << 4));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->bp_free[sp]);
+                if (it >= RING && !(ok = wait_warp(&ctl->done[s], ((it / RING) & 1) ^ 1, ctl, 27))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t o[32];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const uint4 v = w[2 * h + j];
+                        expand_word(v.x, o + 16 * j);
+                        expand_word(v.y, o + 16 * j + 4);
+                        expand_word(v.z, o + 16 * j + 8);
+                        expand_word(v.w, o + 16 * j + 12);
+                    }
+                    tmem_st32(tmem + lanes + kTmemA + s * 64 + h * 32, o);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->a_full[s]);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
+        // ==================================================================== epilogue
+        // warp: lanes 32 q .. of the accumulators, 16-column chunks half, half + 2, ... of the tile
+        const int q = warp & 3, half = (warp - EPI_WARP0) >> 2, row = q * 32 + lane;
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        int it = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+            const Unit un = find_unit(p, u, kCols, tiles, ends);
+            const int n0 = un.tile * ROWS;
+            const int nrow = GATED ? (row < 64 ? n0 + row : p.N + n0 + row - 64) : n0 + row;     // weight row of the expert
+            const bool live = GATED ? n0 + (row & 63) < p.N : n0 + row < p.N;
+            const size_t wrow = (size_t)un.expert * (GATED ? 2 * p.N : p.N) + nrow;
+            const __half* sa = p.ws + (live ? wrow : 0) * G;
+            float C[4][16];
+#pragma unroll
+            for (int a = 0; a < 4; a++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) C[a][j] = 0.f;
+            float s_next = __half2float(sa[0]);
+            for (int g = 0; g < G; g++, it++) {
+                const float s = s_next;
+                s_next = __half2float(sa[g + 1 < G ? g + 1 : g]);
+                const float* sb = sring + (it % SLOTS) * kCols + half * 16;
+                if (!(ok = wait_warp(&ctl->done[it % RING], (it / RING) & 1, ctl, 28))) break;
+                tc_fence_after();
+                const uint32_t d = tmem + lanes + (it & 1) * kCols + half * 16;
+#pragma unroll
+                for (int a = 0; a < 4; a++) {
+                    if (a * 32 + half * 16 >= un.count) break;
+                    uint32_t r[16];
+                    tmem_ld16(d + a * 32, r);
+                    float f[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const float4 b = *reinterpret_cast<const float4*>(sb + a * 32 + j);
+                        mul2(f[j], f[j + 1], s, b.x, b.y);
+                        mul2(f[j + 2], f[j + 3], s, b.z, b.w);
+                    }
+                    tmem_ld_wait16(r);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) fma2(C[a][j], C[a][j + 1], __uint_as_float(r[j]), __uint_as_float(r[j + 1]), f[j], f[j + 1]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->acc_free[it & 1]);
+            }
+            if (!ok) break;
+            const float* bias = p.bias ? p.bias + (size_t)un.expert * (GATED ? 2 * p.N : p.N) : nullptr;
+            if (GATED) {
+                if (row >= 64) {
+#pragma unroll
+                    for (int a = 0; a < 4; a++)
+#pragma unroll
+                        for (int j = 0; j < 16; j++) xch[(a * 32 + half * 16 + j) * 64 + row - 64] = C[a][j];
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (row < 64 && live) {
+#pragma unroll
+                    for (int a = 0; a < 4; a++)
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const int col = a * 32 + half * 16 + j;
+                            if (col < un.count) finish_gated(p, bias, (size_t)un.first + col, n0 + row, C[a][j], xch[col * 64 + row]);
+                        }
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+            } else if (live) {
+#pragma unroll
+                for (int a = 0; a < 4; a++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const int col = a * 32 + half * 16 + j;
+                        if (col < un.count) finish(p, bias, (size_t)un.first + col, n0 + row, C[a][j]);
+                    }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == MMA_WARP) tmem_dealloc(tmem, kTmemCols);
+    pdl_launch_dependents();
+}
+
+size_t smem_bytes(const Params& p) {
+    return 1024 + RING * B_BYTES + BP * BP_BYTES + SLOTS * kCols * 4 + (p.gated ? kCols * 64 * 4 : 0) + sizeof(Control) + (size_t)p.n_exp * 4;
+}
+
+}  // namespace
+
+int run_tiles(const char* kn, const LaunchCtx& c, const Params& p) {
+    const long long xrows = p.offsets ? p.xrows : p.m;
+    FM_REQUIRE((unsigned long long)xrows * (p.K / 8) < 0xffffffffull, kn, "%lld rows of %d values are too many for one call", xrows, p.K);
+    const size_t bytes = (size_t)xrows * p.K * 2;
+    __half* xh = static_cast<__half*>(engine_scratch(bytes));
+    FM_REQUIRE(xh, kn, "the engine workspace cannot grow to %zu bytes here (inside a capture: raise FM_SCRATCH_MB)", bytes);
+    CUtensorMap map;
+    const uint64_t wrows = (uint64_t)p.n_exp * p.N * (p.gated ? 2 : 1);
+    FM_REQUIRE(wrows < 0x7fffffff && encode_bytes_box_map(&map, p.wq, wrows, (uint64_t)p.K / 2, 64, 64), kn,
+               "the tensor map of %llu rows of %d bytes was refused", (unsigned long long)wrows, p.K / 2);
+    const size_t n = (size_t)xrows * (p.K / 16);
+    size_t eb = (n + 255) / 256;
+    if (eb > (size_t)c.sm_count * 16) eb = (size_t)c.sm_count * 16;
+    cudaError_t e = launch_kernel(expand_codes_kernel, dim3((unsigned)eb), dim3(256), 0, c.stream, pdl_enabled(), reinterpret_cast<const uint2*>(p.ae),
+                                  reinterpret_cast<const uint2*>(p.ao), reinterpret_cast<uint4*>(xh), n);
+    if (e != cudaSuccess) return cuda_fail(kn, e);
+    const int rc = after_launch(kn);
+    if (rc != FM_OK) return rc;
+    auto kern = p.gated ? tile_kernel<true> : tile_kernel<false>;
+    const size_t smem = smem_bytes(p);
+    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return cuda_fail(kn, e);
+    const int rows = p.gated ? 64 : 128;
+    long long chunks = (p.m + kCols - 1) / kCols;
+    if (p.offsets) chunks = chunks + p.n_exp < p.m ? chunks + p.n_exp : p.m;
+    const long long units = chunks * ((p.N + rows - 1) / rows);
+    FM_REQUIRE(units < (1ll << 30), kn, "%lld tiles are too many for one call", units);
+    const unsigned grid = (unsigned)(units < c.sm_count ? units : c.sm_count);
+    e = launch_kernel(kern, dim3(grid), dim3(kThreads), smem, c.stream, pdl_enabled(), map, p, (const __half*)xh);
+    return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
+}
+
+}  // namespace linear
+
+int linear_read_status() {
+    int v = 0;
+    const int zero = 0;
+    if (cudaMemcpyFromSymbol(&v, linear::g_status, sizeof(int)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(linear::g_status, &zero, sizeof(int));
+    return v;
+}
+
+}  // namespace fm
