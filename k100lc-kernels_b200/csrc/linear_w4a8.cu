@@ -123,20 +123,22 @@ rows_kernel(const Params p, int wk) {
         }
         if (live && part == 0) {
             const float* bias = p.bias ? p.bias + (size_t)un.expert * (GATED ? 2 * p.N : p.N) : nullptr;
+            const int na = n0 + fr, nb = GATED ? p.N + na : na + 8;   // the lane's two weight rows
+            const bool has_a = na < p.N, has_b = GATED ? has_a : nb < p.N;
+            const float ba = bias && has_a ? bias[na] : 0.f, bb = bias && has_b ? bias[nb] : 0.f;
+            const long long end = (long long)un.first + un.count;
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int c = t * 8 + fq * 2 + h;
-                    if (c >= un.count) continue;
-                    const size_t m = (size_t)un.first + c;
-                    if (GATED) {
-                        if (n0 + fr < p.N) finish_gated(p, bias, m, n0 + fr, acc[t][h], acc[t][2 + h]);
-                    } else {
-                        if (n0 + fr < p.N) finish(p, bias, m, n0 + fr, acc[t][h]);
-                        if (n0 + 8 + fr < p.N) finish(p, bias, m, n0 + 8 + fr, acc[t][2 + h]);
-                    }
+            for (int t = 0; t < NT; t++) {
+                const long long m = (long long)un.first + t * 8 + fq * 2;
+                float v[2] = {acc[t][0] + ba, acc[t][1] + ba}, w[2] = {acc[t][2] + bb, acc[t][3] + bb};
+                if (m >= end) continue;
+                if (GATED) {
+                    if (has_a) finish<2, true>(p, m, 1, end, na, v, w);
+                } else {
+                    if (has_a) finish<2, false>(p, m, 1, end, na, v, v);
+                    if (has_b) finish<2, false>(p, m, 1, end, nb, w, w);
                 }
+            }
         }
     }
     pdl_launch_dependents();

@@ -27,29 +27,46 @@ struct Params {
     bool gated;
 };
 
-__device__ __forceinline__ float activate(int act, float v) {
+// exp and erfc to two or three units in the last place, the reciprocal correctly rounded: a few 2^-24 of the result
+template <int ACT>
+__device__ __forceinline__ float activate(float v) {
+    if (ACT == 1) return v < 0.f ? 0.f : v;                          // (NaN stays NaN)
+    if (ACT == 2) return v * __frcp_rn(1.f + expf(-v));
+    if (ACT == 3) return 0.5f * v * erfcf(v * -0.70710678f);         // 1 + erf(t) = erfc(-t): no cancellation for v < 0
+    if (ACT == 4) return v * __frcp_rn(1.f + expf(-1.5957691f * (v + 0.044715f * v * v * v)));   // 1 + tanh(t) = 2 / (1 + exp(-2t))
+    return v;
+}
+template <int ACT, int N>
+__device__ __forceinline__ void activate_all(float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = activate<ACT>(v[i]);
+}
+// N values at a time, so that the choice of the activation is one branch and the values overlap
+template <int N>
+__device__ __forceinline__ void activate_n(int act, float (&v)[N]) {
     switch (act) {
-        case 1: return v < 0.f ? 0.f : v;                               // (NaN stays NaN)
-        case 2: return __fdiv_rn(v, 1.f + expf(-v));
-        case 3: return 0.5f * v * erfcf(v * -0.70710678f);                // 1 + erf(t) = erfc(-t): no cancellation for v < 0
-        case 4: return __fdiv_rn(v, 1.f + expf(-1.5957691f * (v + 0.044715f * v * v * v)));   // 1 + tanh(t) = 2 / (1 + exp(-2t))
-        default: return v;
+        case 1: activate_all<1>(v); break;
+        case 2: activate_all<2>(v); break;
+        case 3: activate_all<3>(v); break;
+        case 4: activate_all<4>(v); break;
+        default: break;
     }
 }
-__device__ __forceinline__ void finish(const Params& p, const float* bias, size_t m, int n, float v) {
-    if (bias) v += bias[n];
-    v = activate(p.act, v);
-    if (p.residual) v += p.residual[m * p.ldr + n];
-    p.y[m * p.ldy + n] = v;
-}
-__device__ __forceinline__ void finish_gated(const Params& p, const float* bias, size_t m, int n, float gate, float up) {
-    if (bias) {
-        gate += bias[n];
-        up += bias[p.N + n];
-    }
-    float v = activate(p.act, gate) * up;
-    if (p.residual) v += p.residual[m * p.ldr + n];
-    p.y[m * p.ldy + n] = v;
+// y[m + i * step, n] for the N sums v (gated: gates v, ups u); rows from `end` on are left alone.  The bias is in the
+// sums already.  All residuals are read before the first value is written: an element is the residual of itself only.
+template <int N, bool GATED>
+__device__ __forceinline__ void finish(const Params& p, long long m, int step, long long end, int n, float (&v)[N], const float (&u)[N]) {
+    float r[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) r[i] = p.residual && m + i * step < end ? p.residual[(m + i * step) * p.ldr + n] : 0.f;
+    activate_n(p.act, v);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        if (m + i * step < end) {
+            float o = GATED ? v[i] * u[i] : v[i];
+            if (p.residual) o += r[i];
+            p.y[(m + i * step) * p.ldy + n] = o;
+        }
 }
 
 // A unit is one tile of weight rows times one chunk of a bucket's rows; units of a chunk differ in the tile last.

@@ -32,7 +32,7 @@ using namespace tc;
 constexpr int kCols = 128;                          // rows of x per tile
 constexpr int RING = 4;                             // stages of A (tensor memory), B (shared memory) and "step done" barriers
 constexpr int BP = 6;                               // stages of packed weights
-constexpr int SLOTS = 8;                            // stages of activation scales (reuse distance: see the loaders)
+constexpr int SLOTS = 8;                            // stages of scales (reuse distance: see the loaders)
 constexpr int kLag = 2;                             // steps between issuing a row fetch and publishing it
 constexpr int B_BYTES = kCols * 256, BP_BYTES = 128 * 64;
 constexpr int MMA_WARP = 1, LOAD_WARP0 = 4, EXP_WARP0 = 8, EPI_WARP0 = 16, kThreads = 24 * 32;
@@ -62,7 +62,6 @@ __device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity, Control* ctl,
     atomicCAS(&g_status, 0, code);
     return false;
 }
-
 // the same by all lanes of a warp, which leave it with one answer (their next instructions are warp-wide)
 __device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, Control* ctl, int code) {
     return __all_sync(0xffffffffu, wait(b, parity, ctl, code));
@@ -118,6 +117,13 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool ta
 }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// weight row of lane `row` of a tile (a row past the end repeats the last one and is not stored)
+template <bool GATED>
+__device__ __forceinline__ size_t weight_row(const Params& p, const Unit& u, int row) {
+    if (!GATED) return (size_t)u.expert * p.N + min(u.tile * 128 + row, p.N - 1);
+    return (size_t)u.expert * 2 * p.N + (row < 64 ? 0 : p.N) + min(u.tile * 64 + (row & 63), p.N - 1);
+}
+
 template <bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
 tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __half* __restrict__ xh) {
@@ -126,8 +132,9 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
     uint8_t* bring = smem;                                           // RING x [2 halves of 64 k][128 rows][128 bytes]
     uint8_t* wring = bring + RING * B_BYTES;                         // BP x [128 rows][64 bytes]
     float* sring = reinterpret_cast<float*>(wring + BP * BP_BYTES);  // SLOTS x [128]
-    float* xch = sring + SLOTS * kCols;                              // [128 columns][64 rows]: up values on their way to the gate lanes
-    Control* ctl = reinterpret_cast<Control*>(xch + (GATED ? kCols * 64 : 0));
+    uint32_t* wsring = reinterpret_cast<uint32_t*>(sring + SLOTS * kCols);   // SLOTS x [128]: the word that holds the weight row's scale
+    float* xch = reinterpret_cast<float*>(wsring + SLOTS * 128);                               // [32 columns][128 rows] of sums on their way out
+    Control* ctl = reinterpret_cast<Control*>(xch + 32 * 128);
     int* ends = reinterpret_cast<int*>(ctl + 1);                     // [n_exp]
     __shared__ Buckets bk;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -211,12 +218,13 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
     } else if (warp < EXP_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
         // ==================================================================== rows of x and their scales
-        // Thread i fetches chunk i % 16 (16 bytes) of the rows i / 16, i / 16 + 8, ..., and the scale of row i.  Slot
+        // Thread i fetches chunk i % 16 (16 bytes) of the rows i / 16, i / 16 + 8, ..., and the scales of row i of x and of
+        // weight row i (the aligned word around it: a copy has at least four bytes, allocations are whole words).  Slot
         // it % SLOTS of the scales was last read by the epilogue of step it - SLOTS: stage it % RING is free when the MMAs of step
         // it - RING have run, which were issued after the accumulator of step it - RING - 2 had been drained.
         const int i = threadIdx.x - LOAD_WARP0 * 32, c = i & 15, r0 = i >> 4;
         const uint32_t dst0 = smem_u32(bring) + (c >> 3) * (kCols * 128) + r0 * 128 + (((c & 7) ^ r0) << 4);
-        const uint32_t sdst0 = smem_u32(sring) + i * 4;
+        const uint32_t sdst0 = smem_u32(sring) + i * 4, wdst0 = smem_u32(wsring) + i * 4;
         int it = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
@@ -230,6 +238,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
             }
             const long long sr = x_row(p, un, i);
             const float* sc = p.asc + (sr < 0 ? 0 : (size_t)sr * G);
+            const __half* wsc = p.ws + weight_row<GATED>(p, un, i) * G;
             const uint4* src = reinterpret_cast<const uint4*>(xh) + c;
             for (int g = 0; g < G; g++, it++, src += 16) {
                 const int s = it % RING;
@@ -239,6 +248,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
                 for (int j = 0; j < 16; j++)
                     if (8 * j < n16) cp_async16(dst + j * 1024, off[j] == ~0u ? src : src + off[j], off[j] != ~0u);
                 cp_async4(sdst0 + (it % SLOTS) * (kCols * 4), sc + g, sr >= 0);
+                cp_async4(wdst0 + (it % SLOTS) * 512, reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(wsc + g) & ~(uintptr_t)3), true);
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if (it >= kLag) {
                     cp_async_wait<kLag>();
@@ -303,22 +313,20 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
             const Unit un = find_unit(p, u, kCols, tiles, ends);
             const int n0 = un.tile * ROWS;
-            const int nrow = GATED ? (row < 64 ? n0 + row : p.N + n0 + row - 64) : n0 + row;     // weight row of the expert
             const bool live = GATED ? n0 + (row & 63) < p.N : n0 + row < p.N;
-            const size_t wrow = (size_t)un.expert * (GATED ? 2 * p.N : p.N) + nrow;
-            const __half* sa = p.ws + (live ? wrow : 0) * G;
+            uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, row) * G) >> 1) & 1;   // half of the word
+            const float bias = p.bias ? p.bias[weight_row<GATED>(p, un, row)] : 0.f;
             float C[4][16];
 #pragma unroll
             for (int a = 0; a < 4; a++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) C[a][j] = 0.f;
-            float s_next = __half2float(sa[0]);
-            for (int g = 0; g < G; g++, it++) {
-                const float s = s_next;
-                s_next = __half2float(sa[g + 1 < G ? g + 1 : g]);
+            for (int g = 0; g < G; g++, it++, odd ^= 1) {
                 const float* sb = sring + (it % SLOTS) * kCols + half * 16;
                 if (!(ok = wait_warp(&ctl->done[it % RING], (it / RING) & 1, ctl, 28))) break;
                 tc_fence_after();
+                const uint32_t sw = wsring[(it % SLOTS) * 128 + row];
+                const float s = __half2float(__ushort_as_half((unsigned short)(odd ? sw >> 16 : sw & 0xffffu)));
                 const uint32_t d = tmem + lanes + (it & 1) * kCols + half * 16;
 #pragma unroll
                 for (int a = 0; a < 4; a++) {
@@ -341,33 +349,38 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
                 if (lane == 0) mbar_arrive(&ctl->acc_free[it & 1]);
             }
             if (!ok) break;
-            const float* bias = p.bias ? p.bias + (size_t)un.expert * (GATED ? 2 * p.N : p.N) : nullptr;
-            if (GATED) {
-                if (row >= 64) {
+            // 32 columns at a time through shared memory, so that the loop with the activation stays rolled: unrolled over
+            // the 64 registers it was 60 KB of code, and fetching that took 1.7 times as long as the tile's products
 #pragma unroll
-                    for (int a = 0; a < 4; a++)
+            for (int a = 0; a < 4; a++) {
+                if (a * 32 >= un.count) break;
 #pragma unroll
-                        for (int j = 0; j < 16; j++) xch[(a * 32 + half * 16 + j) * 64 + row - 64] = C[a][j];
-                }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (row < 64 && live) {
+                for (int j = 0; j < 16; j++) xch[(half * 16 + j) * 128 + row] = C[a][j] + bias;
+                const long long m0 = (long long)un.first + a * 32, end = (long long)un.first + un.count;
+                if (GATED) {                                         // gate lane r meets up lane 64 + r
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    const int t = threadIdx.x - EPI_WARP0 * 32, r = t & 63;
+                    if (n0 + r < p.N)
+#pragma unroll 1
+                        for (int col = t >> 6; col < 32 && m0 + col < end; col += 16) {
+                            float v[4], up[4];
 #pragma unroll
-                    for (int a = 0; a < 4; a++)
-#pragma unroll
-                        for (int j = 0; j < 16; j++) {
-                            const int col = a * 32 + half * 16 + j;
-                            if (col < un.count) finish_gated(p, bias, (size_t)un.first + col, n0 + row, C[a][j], xch[col * 64 + row]);
+                            for (int i = 0; i < 4; i++) {
+                                v[i] = xch[(col + 4 * i) * 128 + r];
+                                up[i] = xch[(col + 4 * i) * 128 + 64 + r];
+                            }
+                            finish<4, true>(p, m0 + col, 4, end, n0 + r, v, up);
                         }
-                }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-            } else if (live) {
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                } else if (live) {                                   // a thread reads what it wrote
+#pragma unroll 1
+                    for (int col = half * 16; col < half * 16 + 16 && m0 + col < end; col += 4) {
+                        float v[4];
 #pragma unroll
-                for (int a = 0; a < 4; a++)
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int col = a * 32 + half * 16 + j;
-                        if (col < un.count) finish(p, bias, (size_t)un.first + col, n0 + row, C[a][j]);
+                        for (int i = 0; i < 4; i++) v[i] = xch[(col + i) * 128 + row];
+                        finish<4, false>(p, m0 + col, 1, end, n0 + row, v, v);
                     }
+                }
             }
         }
     }
@@ -378,7 +391,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
 }
 
 size_t smem_bytes(const Params& p) {
-    return 1024 + RING * B_BYTES + BP * BP_BYTES + SLOTS * kCols * 4 + (p.gated ? kCols * 64 * 4 : 0) + sizeof(Control) + (size_t)p.n_exp * 4;
+    return 1024 + RING * B_BYTES + BP * BP_BYTES + SLOTS * (kCols + 128) * 4 + 32 * 128 * 4 + sizeof(Control) + (size_t)p.n_exp * 4;
 }
 
 }  // namespace
