@@ -9,13 +9,14 @@
 // times as long as the MMAs).
 //
 // Roles of the 24 warps of the persistent CTA, joined by mbarriers (every wait is bounded):
-//   * one lane copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring;
+//   * one warp copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring;
 //   * eight warps expand them: a thread owns a weight row, reads its 64 bytes, turns nibbles into f16 pairs with four
 //     logic and four arithmetic instructions a word, and writes them to tensor memory, from where the MMA takes its A
 //     operand: no shared-memory traffic for the wide operand, which would otherwise bound the tile (128 bytes a clock);
-//   * four warps fetch the rows of x (f16, expanded once per call by a small kernel in front, k in the order of the
-//     nibble pairs) with 16-byte cp.async, gathering them by the plan, into the 128-byte-swizzled layout of B;
-//   * two threads issue the MMAs of the even and the odd groups into two accumulators;
+//   * one warp copies the rows of x by TMA: f16, put into bucket order and into the k order of the nibble pairs once per
+//     call by a small kernel in front;
+//   * four warps fetch the scales of the weight rows and of the rows of x (cp.async);
+//   * two warps issue the MMAs of the even and the odd groups into two accumulators;
 //   * eight warps drain the accumulators: C[m, n] = fmaf(float(I), ws * asc, C) in registers, then the epilogue.
 #include <cuda.h>
 
@@ -33,12 +34,12 @@ constexpr int kCols = 128;                          // rows of x per tile
 constexpr int RING = 4;                             // stages of A (tensor memory), B (shared memory) and "step done" barriers
 constexpr int BP = 6;                               // stages of packed weights
 constexpr int SLOTS = 8;                            // stages of scales (reuse distance: see the loaders)
-constexpr int kLag = 2;                             // steps between issuing a row fetch and publishing it
+constexpr int kLag = 2;                             // steps between issuing a fetch of scales and publishing it
 constexpr int B_BYTES = kCols * 256, BP_BYTES = 128 * 64;
-constexpr int MMA_WARP = 1, LOAD_WARP0 = 4, EXP_WARP0 = 8, EPI_WARP0 = 16, kThreads = 24 * 32;
+constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 3, SCALE_WARP0 = 4, EXP_WARP0 = 8, EPI_WARP0 = 16, kThreads = 24 * 32;
 // 768 threads start with 80 registers each (61 440 of the file); the shares below add up to the same
-constexpr int kRegsIssue = 32, kRegsLoad = 64, kRegsExpand = 72, kRegsEpilogue = 120;
-static_assert(kRegsIssue + kRegsLoad + 2 * kRegsExpand + 2 * kRegsEpilogue == 480, "register shares of the six warpgroups");
+constexpr int kRegsIssue = 48, kRegsScale = 40, kRegsExpand = 72, kRegsEpilogue = 120;
+static_assert(kRegsIssue + kRegsScale + 2 * kRegsExpand + 2 * kRegsEpilogue <= 480, "register shares of the six warpgroups");
 static_assert(SLOTS >= RING + 2, "a scale slot is rewritten RING steps ahead of the MMAs, which are 2 ahead of the epilogue");
 constexpr int kSpin = 1 << 17;
 constexpr uint32_t kTmemCols = 512, kTmemA = 256;   // accumulators: columns 0..255; A: 4 x 64 columns
@@ -64,6 +65,7 @@ __device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity, Control* ctl,
 }
 // the same by all lanes of a warp, which leave it with one answer (their next instructions are warp-wide)
 __device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, Control* ctl, int code) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return true;
     return __all_sync(0xffffffffu, wait(b, parity, ctl, code));
 }
 
@@ -90,12 +92,24 @@ __device__ __forceinline__ void expand_word(uint32_t w, uint32_t* o) {
     o[3] = fma_f16x2((v & 0x00F000F0u) ^ 0x64806480u, 0x2C002C00u, 0xD480D480u);
 }
 
-// codes [rows][K/2] even and odd -> f16 [rows][K] in the pair order above
+// codes [xrows][K/2] even and odd -> f16 [m][K] in the pair order above; slot s of a plan takes row bucket_rows[s].  A thread
+// turns 16 k; slots behind the last bucket and slots of no row are skipped.
 __global__ void __launch_bounds__(256)
-expand_codes_kernel(const uint2* __restrict__ ae, const uint2* __restrict__ ao, uint4* __restrict__ out, size_t n) {
+expand_codes_kernel(const Params p, __half* __restrict__ out) {
     pdl_wait();
-    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
-        const uint2 e = ae[i], o = ao[i];                            // 16 k
+    const int per_row = p.K / 16;
+    const long long used = p.offsets ? bound(p, p.n_exp) : p.m, n = used * per_row;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+        const long long slot = i / per_row;
+        const int c = (int)(i - slot * per_row);
+        long long row = slot;
+        if (p.bucket_rows) {
+            row = p.bucket_rows[slot];
+            if (row < 0 || row >= p.xrows) continue;
+        }
+        const uint2 e = *reinterpret_cast<const uint2*>(p.ae + row * (p.K / 2) + c * 8);
+        const uint2 o = *reinterpret_cast<const uint2*>(p.ao + row * (p.K / 2) + c * 8);
+        uint4* dst = reinterpret_cast<uint4*>(out + slot * p.K + c * 16);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const uint32_t a = h ? e.y : e.x, b = h ? o.y : o.x;
@@ -103,15 +117,12 @@ expand_codes_kernel(const uint2* __restrict__ ae, const uint2* __restrict__ ao, 
                 const __half2 v = __floats2half2_rn((float)(int8_t)(w >> (8 * j)), (float)(int8_t)(w >> (8 * j + 16)));
                 return *reinterpret_cast<const uint32_t*>(&v);
             };
-            out[2 * i + h] = make_uint4(pair(a, 0), pair(b, 0), pair(a, 1), pair(b, 1));
+            dst[h] = make_uint4(pair(a, 0), pair(b, 0), pair(a, 1), pair(b, 1));
         }
     }
     pdl_launch_dependents();
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool take) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
 }
@@ -124,16 +135,32 @@ __device__ __forceinline__ size_t weight_row(const Params& p, const Unit& u, int
     return (size_t)u.expert * 2 * p.N + (row < 64 ? 0 : p.N) + min(u.tile * 64 + (row & 63), p.N - 1);
 }
 
+// Position in a ring of N stages and the parity of its phase there.
+template <int N>
+struct Ring {
+    int s = 0;
+    uint32_t ph = 0;
+    __device__ __forceinline__ void next() {
+        if (++s == N) {
+            s = 0;
+            ph ^= 1;
+        }
+    }
+};
+
+struct RowMaps { CUtensorMap box[4]; };             // boxes of 128, 64, 32 and 16 rows of x (64 k)
+
+// GATED: 64 gate rows and 64 up rows make a tile.
 template <bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
-tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __half* __restrict__ xh) {
+tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ RowMaps map_x, const Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* bring = smem;                                           // RING x [2 halves of 64 k][128 rows][128 bytes]
     uint8_t* wring = bring + RING * B_BYTES;                         // BP x [128 rows][64 bytes]
     float* sring = reinterpret_cast<float*>(wring + BP * BP_BYTES);  // SLOTS x [128]
     uint32_t* wsring = reinterpret_cast<uint32_t*>(sring + SLOTS * kCols);   // SLOTS x [128]: the word that holds the weight row's scale
-    float* xch = reinterpret_cast<float*>(wsring + SLOTS * 128);                               // [32 columns][128 rows] of sums on their way out
+    float* xch = reinterpret_cast<float*>(wsring + SLOTS * 128);     // [32 columns][128 rows] of sums on their way out
     Control* ctl = reinterpret_cast<Control*>(xch + 32 * 128);
     int* ends = reinterpret_cast<int*>(ctl + 1);                     // [n_exp]
     __shared__ Buckets bk;
@@ -148,7 +175,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
         }
         for (int i = 0; i < RING; i++) {
             mbar_init(&ctl->a_full[i], 4);
-            mbar_init(&ctl->b_full[i], 4);
+            mbar_init(&ctl->b_full[i], 5);
             mbar_init(&ctl->done[i], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -166,122 +193,149 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
     pdl_wait();
     const int total = count_units(p, kCols, tiles, ends, &bk);
 
-    if (warp < LOAD_WARP0) {
+    if (warp < SCALE_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
-        if (warp == 0 && lane == 0) {
+        // In these roles the whole warp walks the steps and one lane is elected to issue: a single lane that waits alone polls
+        // its barrier dozens of times a step, and descriptors stay in uniform registers.
+        if (warp == WEIGHT_WARP) {
             // ================================================================ packed weights
+            Ring<BP> r;
             int it = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const int y0 = un.expert * (GATED ? 2 * p.N : p.N) + un.tile * ROWS, y1 = y0 + (GATED ? p.N : 64);
-                for (int g = 0; g < G; g++, it++) {
-                    const int s = it % BP;
-                    if (it >= BP && !(ok = wait(&ctl->bp_free[s], ((it / BP) & 1) ^ 1, ctl, 21))) break;
-                    mbar_expect_tx(&ctl->bp_full[s], BP_BYTES);
-                    tma_2d(wring + s * BP_BYTES, &map, g * 64, y0, &ctl->bp_full[s]);
-                    tma_2d(wring + s * BP_BYTES + BP_BYTES / 2, &map, g * 64, y1, &ctl->bp_full[s]);
+                for (int g = 0; g < G; g++, it++, r.next()) {
+                    if (it >= BP && !(ok = wait_warp(&ctl->bp_free[r.s], r.ph ^ 1, ctl, 21))) break;
+                    if (elect_one()) {
+                        mbar_expect_tx(&ctl->bp_full[r.s], BP_BYTES);
+                        tma_2d(wring + r.s * BP_BYTES, &map_w, g * 64, y0, &ctl->bp_full[r.s]);
+                        tma_2d(wring + r.s * BP_BYTES + BP_BYTES / 2, &map_w, g * 64, y1, &ctl->bp_full[r.s]);
+                    }
+                    __syncwarp();
                 }
             }
             if (ctl->abort)                                          // copies in flight land before the memory is given up
                 for (int j = it > BP ? it - BP : 0; j < it; j++)
                     for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->bp_full[j % BP], (j / BP) & 1); i++) {}
-        } else if ((warp == MMA_WARP || warp == MMA_WARP + 1) && lane == 0) {
+        } else if (warp == ROW_WARP) {
+            // ================================================================ rows of x
+            // A count of rows is a sum of boxes of 128, 64, 32 and 16: a box costs its issue, about 100 clocks, whatever it holds
+            // (16-row boxes throughout, 16 instructions a step, bound the tile at 1800 clocks; four-row gathers at 6000)
+            Ring<RING> r;
+            int it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+                const Unit un = find_unit(p, u, kCols, tiles, ends);
+                const int n16 = (un.count + 15) & ~15;
+                for (int g = 0; g < G; g++, it++, r.next()) {
+                    if (it >= RING && !(ok = wait_warp(&ctl->done[r.s], r.ph ^ 1, ctl, 25))) break;
+                    uint64_t* bar = &ctl->b_full[r.s];
+                    if (elect_one()) {
+                        mbar_expect_tx(bar, (uint32_t)n16 * 256);
+                        uint8_t* dst = bring + r.s * B_BYTES;
+                        int at = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; b++)
+                            if (n16 & (128 >> b)) {
+                                tma_2d(dst + at * 128, &map_x.box[b], g * 256, un.first + at, bar);
+                                tma_2d(dst + at * 128 + kCols * 128, &map_x.box[b], g * 256 + 128, un.first + at, bar);
+                                at += 128 >> b;
+                            }
+                    }
+                    __syncwarp();
+                }
+            }
+            if (ctl->abort)
+                for (int j = it > RING ? it - RING : 0; j < it; j++)
+                    for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->b_full[j % RING], (j / RING) & 1); i++) {}
+        } else {
             // ================================================================ MMA issuers: even and odd steps
             const int par = warp - MMA_WARP;
             const uint64_t bdesc0 = smem_desc_sw128(smem_u32(bring));
+            Ring<RING> r;
             int it = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const uint32_t idesc = instr_desc((un.count + 15) & ~15);
-                for (int g = 0; g < G; g++, it++) {
+                for (int g = 0; g < G; g++, it++, r.next()) {
                     if ((it & 1) != par) continue;
-                    const int s = it % RING;
-                    const uint32_t ph = (it / RING) & 1;
-                    if (it >= 2 && !(ok = wait(&ctl->acc_free[par], ((it >> 1) & 1) ^ 1, ctl, 22))) break;
-                    if (!(ok = wait(&ctl->a_full[s], ph, ctl, 23))) break;
-                    if (!(ok = wait(&ctl->b_full[s], ph, ctl, 24))) break;
+                    if (!(ok = wait_warp(&ctl->a_full[r.s], r.ph, ctl, 23))) break;
+                    if (!(ok = wait_warp(&ctl->b_full[r.s], r.ph, ctl, 24))) break;
+                    if (it >= 2 && !(ok = wait_warp(&ctl->acc_free[par], ((it >> 1) & 1) ^ 1, ctl, 22))) break;
                     tc_fence_after();
-                    const uint64_t bd = bdesc0 + (uint64_t)(s * (B_BYTES >> 4));
-                    const uint32_t d = tmem + par * kCols, a = tmem + kTmemA + s * 64;
+                    const uint64_t bd = bdesc0 + (uint64_t)(r.s * (B_BYTES >> 4));
+                    const uint32_t d = tmem + par * kCols, a = tmem + kTmemA + r.s * 64;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++)                      // 16 k each: 8 columns of A, 32 bytes of B
-                        tc_mma_f16_ts(d, a + j * 8, bd + (j >> 2) * (kCols * 128 >> 4) + (j & 3) * 2, idesc, j > 0);
-                    tc_commit(&ctl->done[s]);
+                        for (int j = 0; j < 8; j++)                  // 16 k each: 8 columns of A, 32 bytes of B
+                            tc_mma_f16_ts(d, a + j * 8, bd + (j >> 2) * (kCols * 128 >> 4) + (j & 3) * 2, idesc, j > 0);
+                        tc_commit(&ctl->done[r.s]);
+                    }
+                    __syncwarp();
                 }
             }
-            // nothing this thread issued may still run when tensor memory is released
-            tc_commit(&ctl->drain[par]);
+            // nothing this warp issued may still run when tensor memory is released (the lane that issued commits: elect.sync
+            // names the same lane of a full warp every time)
+            if (elect_one()) tc_commit(&ctl->drain[par]);
             for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->drain[par], 0); i++) {}
         }
     } else if (warp < EXP_WARP0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
-        // ==================================================================== rows of x and their scales
-        // Thread i fetches chunk i % 16 (16 bytes) of the rows i / 16, i / 16 + 8, ..., and the scales of row i of x and of
-        // weight row i (the aligned word around it: a copy has at least four bytes, allocations are whole words).  Slot
-        // it % SLOTS of the scales was last read by the epilogue of step it - SLOTS: stage it % RING is free when the MMAs of step
-        // it - RING have run, which were issued after the accumulator of step it - RING - 2 had been drained.
-        const int i = threadIdx.x - LOAD_WARP0 * 32, c = i & 15, r0 = i >> 4;
-        const uint32_t dst0 = smem_u32(bring) + (c >> 3) * (kCols * 128) + r0 * 128 + (((c & 7) ^ r0) << 4);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsScale));
+        // ==================================================================== scales
+        // Thread i fetches the scale of row i of x and the aligned word around that of weight row i (a copy has at least four
+        // bytes; allocations are whole words).  Slot it % SLOTS was last read by the epilogue of step it - SLOTS: stage
+        // it % RING is free when the MMAs of step it - RING have run, which were issued after the accumulator of step
+        // it - RING - 2 had been drained.
+        const int i = threadIdx.x - SCALE_WARP0 * 32;
         const uint32_t sdst0 = smem_u32(sring) + i * 4, wdst0 = smem_u32(wsring) + i * 4;
+        Ring<RING> r, behind;
         int it = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
             const Unit un = find_unit(p, u, kCols, tiles, ends);
-            const int n16 = (un.count + 15) & ~15;
-            uint32_t off[16];                                        // rows in units of 16 bytes; ~0: zeros
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const long long r = r0 + 8 * j < n16 ? x_row(p, un, r0 + 8 * j) : -1;
-                off[j] = r < 0 ? ~0u : (uint32_t)(r * (p.K / 8));
-            }
             const long long sr = x_row(p, un, i);
             const float* sc = p.asc + (sr < 0 ? 0 : (size_t)sr * G);
             const __half* wsc = p.ws + weight_row<GATED>(p, un, i) * G;
-            const uint4* src = reinterpret_cast<const uint4*>(xh) + c;
-            for (int g = 0; g < G; g++, it++, src += 16) {
-                const int s = it % RING;
-                if (it >= RING && !(ok = wait_warp(&ctl->done[s], ((it / RING) & 1) ^ 1, ctl, 25))) break;
-                const uint32_t dst = dst0 + s * B_BYTES;
-#pragma unroll
-                for (int j = 0; j < 16; j++)
-                    if (8 * j < n16) cp_async16(dst + j * 1024, off[j] == ~0u ? src : src + off[j], off[j] != ~0u);
+            for (int g = 0; g < G; g++, it++, r.next()) {
+                if (it >= RING && !(ok = wait_warp(&ctl->done[r.s], r.ph ^ 1, ctl, 29))) break;
                 cp_async4(sdst0 + (it % SLOTS) * (kCols * 4), sc + g, sr >= 0);
                 cp_async4(wdst0 + (it % SLOTS) * 512, reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(wsc + g) & ~(uintptr_t)3), true);
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if (it >= kLag) {
                     cp_async_wait<kLag>();
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&ctl->b_full[(it - kLag) % RING]);
+                    if (lane == 0) mbar_arrive(&ctl->b_full[behind.s]);
+                    behind.next();
                 }
             }
         }
         cp_async_wait<0>();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (ok && lane == 0)
-            for (int j = it > kLag ? it - kLag : 0; j < it; j++) mbar_arrive(&ctl->b_full[j % RING]);
+            for (int j = it > kLag ? it - kLag : 0; j < it; j++, behind.next()) mbar_arrive(&ctl->b_full[behind.s]);
     } else if (warp < EPI_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsExpand));
         // ==================================================================== expansion of the weights
         const int set = (warp - EXP_WARP0) >> 2, q = warp & 3, row = q * 32 + lane;
-        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        const uint32_t a0 = tmem + ((uint32_t)(q * 32) << 16) + kTmemA;
+        const uint8_t* w0 = wring + row * 64;
+        const int x = ((row >> 1) & 3) << 4;                         // 64-byte swizzle: chunk ^= (row / 2) % 4
+        Ring<BP> rp;
+        Ring<RING> r;
         int it = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
-            for (int g = 0; g < G; g++, it++) {
+            for (int g = 0; g < G; g++, it++, rp.next(), r.next()) {
                 if ((it & 1) != set) continue;
-                const int sp = it % BP, s = it % RING;
-                if (!(ok = wait_warp(&ctl->bp_full[sp], (it / BP) & 1, ctl, 26))) break;
+                if (!(ok = wait_warp(&ctl->bp_full[rp.s], rp.ph, ctl, 26))) break;
                 uint4 w[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++)                          // 64-byte swizzle: chunk ^= (row / 2) % 4
-                    w[j] = *reinterpret_cast<const uint4*>(wring + sp * BP_BYTES + row * 64 + ((j ^ ((row >> 1) & 3)) << 4));
+                for (int j = 0; j < 4; j++) w[j] = *reinterpret_cast<const uint4*>(w0 + rp.s * BP_BYTES + ((j << 4) ^ x));
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->bp_free[sp]);
-                if (it >= RING && !(ok = wait_warp(&ctl->done[s], ((it / RING) & 1) ^ 1, ctl, 27))) break;
+                if (lane == 0) mbar_arrive(&ctl->bp_free[rp.s]);
+                if (it >= RING && !(ok = wait_warp(&ctl->done[r.s], r.ph ^ 1, ctl, 27))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -294,12 +348,12 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
                         expand_word(v.z, o + 16 * j + 8);
                         expand_word(v.w, o + 16 * j + 12);
                     }
-                    tmem_st32(tmem + lanes + kTmemA + s * 64 + h * 32, o);
+                    tmem_st32(a0 + r.s * 64 + h * 32, o);
                 }
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->a_full[s]);
+                if (lane == 0) mbar_arrive(&ctl->a_full[r.s]);
             }
         }
     } else {
@@ -307,42 +361,40 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
         // ==================================================================== epilogue
         // warp: lanes 32 q .. of the accumulators, 16-column chunks half, half + 2, ... of the tile
         const int q = warp & 3, half = (warp - EPI_WARP0) >> 2, row = q * 32 + lane;
-        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        const uint32_t d0 = tmem + ((uint32_t)(q * 32) << 16) + half * 16;
+        Ring<RING> r;
         int it = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
             const Unit un = find_unit(p, u, kCols, tiles, ends);
-            const int n0 = un.tile * ROWS;
-            const bool live = GATED ? n0 + (row & 63) < p.N : n0 + row < p.N;
+            const int n0 = un.tile * ROWS, chunks = (un.count - half * 16 + 31) >> 5;
             uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, row) * G) >> 1) & 1;   // half of the word
-            const float bias = p.bias ? p.bias[weight_row<GATED>(p, un, row)] : 0.f;
-            float C[4][16];
+            uint64_t C[4][8];                                        // pairs of neighbouring columns
 #pragma unroll
             for (int a = 0; a < 4; a++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) C[a][j] = 0.f;
-            for (int g = 0; g < G; g++, it++, odd ^= 1) {
+                for (int j = 0; j < 8; j++) C[a][j] = 0;
+            for (int g = 0; g < G; g++, it++, odd ^= 1, r.next()) {
                 const float* sb = sring + (it % SLOTS) * kCols + half * 16;
-                if (!(ok = wait_warp(&ctl->done[it % RING], (it / RING) & 1, ctl, 28))) break;
+                if (!(ok = wait_warp(&ctl->done[r.s], r.ph, ctl, 28))) break;
                 tc_fence_after();
+                const uint32_t d = d0 + (it & 1) * kCols;
                 const uint32_t sw = wsring[(it % SLOTS) * 128 + row];
-                const float s = __half2float(__ushort_as_half((unsigned short)(odd ? sw >> 16 : sw & 0xffffu)));
-                const uint32_t d = tmem + lanes + (it & 1) * kCols + half * 16;
+                const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(odd ? sw >> 16 : sw & 0xffffu))));
+                const uint64_t s2 = pack2(s, s);
 #pragma unroll
                 for (int a = 0; a < 4; a++) {
-                    if (a * 32 + half * 16 >= un.count) break;
-                    uint32_t r[16];
-                    tmem_ld16(d + a * 32, r);
-                    float f[16];
+                    if (a >= chunks) break;
+                    uint64_t f[8], v[8];
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        const float4 b = *reinterpret_cast<const float4*>(sb + a * 32 + j);
-                        mul2(f[j], f[j + 1], s, b.x, b.y);
-                        mul2(f[j + 2], f[j + 3], s, b.z, b.w);
+                    for (int j = 0; j < 8; j += 2) {
+                        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sb + a * 32 + 2 * j);
+                        f[j] = mul2p(s2, b.x);
+                        f[j + 1] = mul2p(s2, b.y);
                     }
-                    tmem_ld_wait16(r);
+                    tmem_ld16_pairs(d + a * 32, v);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) fma2(C[a][j], C[a][j + 1], __uint_as_float(r[j]), __uint_as_float(r[j + 1]), f[j], f[j + 1]);
+                    for (int j = 0; j < 8; j++) fma2p(C[a][j], v[j], f[j]);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -350,29 +402,33 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
             }
             if (!ok) break;
             // 32 columns at a time through shared memory, so that the loop with the activation stays rolled: unrolled over
-            // the 64 registers it was 60 KB of code, and fetching that took 1.7 times as long as the tile's products
+            // the registers it was 60 KB of code, and fetching that took 1.7 times as long as the tile's products
+            const float bias = p.bias ? p.bias[weight_row<GATED>(p, un, row)] : 0.f;
 #pragma unroll
             for (int a = 0; a < 4; a++) {
                 if (a * 32 >= un.count) break;
-#pragma unroll
-                for (int j = 0; j < 16; j++) xch[(half * 16 + j) * 128 + row] = C[a][j] + bias;
                 const long long m0 = (long long)un.first + a * 32, end = (long long)un.first + un.count;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    xch[(half * 16 + 2 * j) * 128 + row] = __uint_as_float((uint32_t)C[a][j]) + bias;
+                    xch[(half * 16 + 2 * j + 1) * 128 + row] = __uint_as_float((uint32_t)(C[a][j] >> 32)) + bias;
+                }
                 if (GATED) {                                         // gate lane r meets up lane 64 + r
                     asm volatile("bar.sync 1, 256;" ::: "memory");
-                    const int t = threadIdx.x - EPI_WARP0 * 32, r = t & 63;
-                    if (n0 + r < p.N)
+                    const int t = threadIdx.x - EPI_WARP0 * 32, gr = t & 63;
+                    if (n0 + gr < p.N)
 #pragma unroll 1
                         for (int col = t >> 6; col < 32 && m0 + col < end; col += 16) {
                             float v[4], up[4];
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                v[i] = xch[(col + 4 * i) * 128 + r];
-                                up[i] = xch[(col + 4 * i) * 128 + 64 + r];
+                                v[i] = xch[(col + 4 * i) * 128 + gr];
+                                up[i] = xch[(col + 4 * i) * 128 + 64 + gr];
                             }
-                            finish<4, true>(p, m0 + col, 4, end, n0 + r, v, up);
+                            finish<4, true>(p, m0 + col, 4, end, n0 + gr, v, up);
                         }
                     asm volatile("bar.sync 1, 256;" ::: "memory");
-                } else if (live) {                                   // a thread reads what it wrote
+                } else if (n0 + row < p.N) {                         // a thread reads what it wrote
 #pragma unroll 1
                     for (int col = half * 16; col < half * 16 + 16 && m0 + col < end; col += 4) {
                         float v[4];
@@ -382,6 +438,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map, const Params p, const __hal
                     }
                 }
             }
+            __syncwarp();
         }
     }
     tc_fence_before();
@@ -397,20 +454,19 @@ size_t smem_bytes(const Params& p) {
 }  // namespace
 
 int run_tiles(const char* kn, const LaunchCtx& c, const Params& p) {
-    const long long xrows = p.offsets ? p.xrows : p.m;
-    FM_REQUIRE((unsigned long long)xrows * (p.K / 8) < 0xffffffffull, kn, "%lld rows of %d values are too many for one call", xrows, p.K);
-    const size_t bytes = (size_t)xrows * p.K * 2;
+    const size_t bytes = (size_t)p.m * p.K * 2;
     __half* xh = static_cast<__half*>(engine_scratch(bytes));
     FM_REQUIRE(xh, kn, "the engine workspace cannot grow to %zu bytes here (inside a capture: raise FM_SCRATCH_MB)", bytes);
-    CUtensorMap map;
+    CUtensorMap map_w;
+    RowMaps map_x;
     const uint64_t wrows = (uint64_t)p.n_exp * p.N * (p.gated ? 2 : 1);
-    FM_REQUIRE(wrows < 0x7fffffff && encode_bytes_box_map(&map, p.wq, wrows, (uint64_t)p.K / 2, 64, 64), kn,
-               "the tensor map of %llu rows of %d bytes was refused", (unsigned long long)wrows, p.K / 2);
-    const size_t n = (size_t)xrows * (p.K / 16);
+    bool ok = wrows < 0x7fffffff && encode_bytes_box_map(&map_w, p.wq, wrows, (uint64_t)p.K / 2, 64, 64);
+    for (int b = 0; b < 4; b++) ok = ok && encode_bytes_box_map(&map_x.box[b], xh, (uint64_t)p.m, (uint64_t)p.K * 2, 128, 128 >> b);
+    FM_REQUIRE(ok, kn, "the tensor maps of %llu rows of weights and %d rows of x were refused (K=%d)", (unsigned long long)wrows, p.m, p.K);
+    const size_t n = (size_t)p.m * (p.K / 16);
     size_t eb = (n + 255) / 256;
     if (eb > (size_t)c.sm_count * 16) eb = (size_t)c.sm_count * 16;
-    cudaError_t e = launch_kernel(expand_codes_kernel, dim3((unsigned)eb), dim3(256), 0, c.stream, pdl_enabled(), reinterpret_cast<const uint2*>(p.ae),
-                                  reinterpret_cast<const uint2*>(p.ao), reinterpret_cast<uint4*>(xh), n);
+    cudaError_t e = launch_kernel(expand_codes_kernel, dim3((unsigned)eb), dim3(256), 0, c.stream, pdl_enabled(), p, xh);
     if (e != cudaSuccess) return cuda_fail(kn, e);
     const int rc = after_launch(kn);
     if (rc != FM_OK) return rc;
@@ -423,7 +479,7 @@ int run_tiles(const char* kn, const LaunchCtx& c, const Params& p) {
     const long long units = chunks * ((p.N + rows - 1) / rows);
     FM_REQUIRE(units < (1ll << 30), kn, "%lld tiles are too many for one call", units);
     const unsigned grid = (unsigned)(units < c.sm_count ? units : c.sm_count);
-    e = launch_kernel(kern, dim3(grid), dim3(kThreads), smem, c.stream, pdl_enabled(), map, p, (const __half*)xh);
+    e = launch_kernel(kern, dim3(grid), dim3(kThreads), smem, c.stream, pdl_enabled(), map_w, map_x, p);
     return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
 }
 

@@ -111,11 +111,33 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
                    "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+// 32 lanes x 16 columns, waited for: thread t gets columns c..c+15 of lane t as eight 64-bit pairs
+__device__ __forceinline__ void tmem_ld16_pairs(uint32_t taddr, uint64_t (&r)[8]) {
+    asm volatile("{\n.reg .b32 t<16>;\n"
+                 "tcgen05.ld.sync.aligned.32x32b.x16.b32 {t0,t1,t2,t3,t4,t5,t6,t7,t8,t9,t10,t11,t12,t13,t14,t15}, [%8];\n"
+                 "tcgen05.wait::ld.sync.aligned;\n"
+                 "mov.b64 %0, {t0,t1};\nmov.b64 %1, {t2,t3};\nmov.b64 %2, {t4,t5};\nmov.b64 %3, {t6,t7};\n"
+                 "mov.b64 %4, {t8,t9};\nmov.b64 %5, {t10,t11};\nmov.b64 %6, {t12,t13};\nmov.b64 %7, {t14,t15};\n}"
+                 : "=l"(r[0]), "=l"(r[1]), "=l"(r[2]), "=l"(r[3]), "=l"(r[4]), "=l"(r[5]), "=l"(r[6]), "=l"(r[7]) : "r"(taddr) : "memory");
 }
+// one lane of a converged warp; the code around the elected instructions stays warp-uniform
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok));
+    return ok != 0;
+}
+// packed fp32 pairs kept in 64-bit registers (no moves around the packed instructions)
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2p(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void fma2p(uint64_t& c, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b)); }
 
 // two fp32 lanes per instruction (sm_100 packed fp32): per lane identical to fmul / fmaf
 __device__ __forceinline__ void mul2(float& d0, float& d1, float a, float b0, float b1) {
