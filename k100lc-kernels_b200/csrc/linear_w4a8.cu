@@ -14,9 +14,14 @@
 //
 // A warp owns 16 weight rows (gated: 8 gate rows and the 8 up rows beside them, so that a lane holds both factors) and
 // multiplies one 128-group at a time with mma.sync m16n8k32, the rows of x being the columns of B.  The four lanes that
-// share a fragment row read the 64 bytes of its group as one 16-byte word each; a word's low and high nibbles are the
-// even and odd k, which is how the codes are stored, so both operands go from memory to the MMA without a shuffle.
-// Nibbles enter as u = nibble ^ 8 (u8 x s8), the accumulators start at -8 * sum(q).
+// share a weight row read the 64 bytes of its group as one 16-byte word each; a word's low and high nibbles are the even
+// and odd k, which is how the codes are stored, so both operands go from memory to the MMA without a shuffle.  Nibbles
+// enter in the upper half of their byte, as the int8 value 16 w (one or two logic instructions a word, no sum of the codes
+// to correct by); the 16 is divided out at the end, exactly.
+// Bound by HBM.  A warp asks for a group of its next chunk (four groups: 256 bytes of every row) as soon as it has multiplied
+// that group of the current one, so that 4 KB a warp are on their way at any time, across the ends of its units too.  Where
+// there are fewer units than warps the K dimension is split over the warps of a team and their partial sums meet in shared
+// memory.
 #include <cuda_fp16.h>
 
 #include "device_utils.cuh"
@@ -27,111 +32,142 @@ namespace fm {
 namespace linear {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kMaxWarps = 8, kCtasPerSm = 2;        // at 128 registers a thread
+constexpr int CH = 4;                               // groups of a chunk
+constexpr int COLS = 8;                             // rows of x of a unit
 
-__device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t lo_u(uint32_t w) { return (w & 0x0F0F0F0Fu) ^ 0x08080808u; }
-__device__ __forceinline__ uint32_t hi_u(uint32_t w) { return ((w >> 4) & 0x0F0F0F0Fu) ^ 0x08080808u; }
+__device__ __forceinline__ void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+// read-once data, and the 256 bytes around it on their way to L2
+__device__ __forceinline__ uint4 ld_stream_256(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t lo16(uint32_t w) { return (w << 4) & 0xF0F0F0F0u; }
+__device__ __forceinline__ uint32_t hi16(uint32_t w) { return w & 0xF0F0F0F0u; }
 __device__ __forceinline__ uint32_t word(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
-// NT: fragments of eight rows of x that share the weights in registers
-template <int NT, bool GATED>
-__global__ void __launch_bounds__(kThreads)
+// wk warps, a team, share a unit; blockDim = 32 * wk * (teams of a CTA), and every team has a run of units of its own.
+// WHOLE: K is a multiple of 512; otherwise the groups past the end of a row repeat its last one with scale 0.
+template <bool GATED, bool WHOLE>
+__global__ void __launch_bounds__(kMaxWarps * 32, kCtasPerSm)
 rows_kernel(const Params p, int wk) {
-    __shared__ float join[kWarps][NT][4][32];
+    __shared__ float join[2][kMaxWarps][4][32];
     __shared__ Buckets bk;
     extern __shared__ int ends[];                                     // [n_exp] units up to and including expert e
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, fr = lane >> 2, fq = lane & 3;
-    constexpr int COLS = 8 * NT, ROWS = GATED ? 8 : 16;
-    const int tiles = (p.N + ROWS - 1) / ROWS, G = p.K / 128;
+    constexpr int ROWS = GATED ? 8 : 16;
+    const int tiles = (p.N + ROWS - 1) / ROWS, G = p.K / 128, chunks = (G + CH - 1) / CH;
     const int total = count_units(p, COLS, tiles, ends, &bk);
-    const int per_cta = kWarps / wk, sub = warp / wk, part = warp % wk;
-    for (int u0 = blockIdx.x * per_cta; u0 < total; u0 += gridDim.x * per_cta) {
-        const int u = u0 + sub;
-        const bool live = u < total;
-        Unit un = {0, 0, 0, 0, 0};
-        if (live) un = find_unit(p, u, COLS, tiles, ends);
-        const int n0 = un.tile * ROWS;
-        float acc[NT][4];
+    const int per_cta = (int)(blockDim.x >> 5) / wk, team = warp / wk, part = warp % wk;
+    const int teams = per_cta * (int)gridDim.x, me = (int)blockIdx.x * per_cta + team;
+    const int c0 = chunks * part / wk, c1 = chunks * (part + 1) / wk;
+    int u = (int)((long long)total * me / teams);
+    const int u1 = (int)((long long)total * (me + 1) / teams);
+    if (u >= u1) return;                                              // (a team's barrier is its own)
+
+    uint4 wa[CH], wb[CH], e[CH], o[CH];
+    unsigned short sa[CH], sb[CH];
+    float f0[CH], f1[CH];                                             // scales of columns 2 fq and 2 fq + 1
+    const uint8_t *pa, *pb;
+    const __half *qa, *qb;
+    const int8_t *xe, *xo;                                            // codes of column fr (no such row: row 0, which is not stored)
+    const float *x0, *x1;
+    auto start = [&](const Unit& n) {                                 // chunk c0 of a unit
+        // (rows past the end repeat the last one and are not stored)
+        const int n0 = n.tile * ROWS, ra = min(n0 + fr, p.N - 1), rb = GATED ? p.N + ra : min(n0 + 8 + fr, p.N - 1), g = c0 * CH;
+        const size_t row0 = (size_t)n.expert * (GATED ? 2 * p.N : p.N);
+        pa = p.wq + (row0 + ra) * (size_t)(p.K / 2) + g * 64 + fq * 16;
+        pb = p.wq + (row0 + rb) * (size_t)(p.K / 2) + g * 64 + fq * 16;
+        qa = p.ws + (row0 + ra) * (size_t)G + g;
+        qb = p.ws + (row0 + rb) * (size_t)G + g;
+        const size_t r = (size_t)max(x_row(p, n, fr), 0ll) * (p.K / 2) + g * 64 + fq * 16;
+        xe = p.ae + r;
+        xo = p.ao + r;
+        x0 = p.asc + (size_t)max(x_row(p, n, 2 * fq), 0ll) * G + g;
+        x1 = p.asc + (size_t)max(x_row(p, n, 2 * fq + 1), 0ll) * G + g;
+    };
+    auto load = [&](int j, int last) {                                // group j of the chunk, whose last group is `last`
+        const int at = WHOLE ? j : min(j, last);
+        wa[j] = ld_stream_256(pa + at * 64);
+        wb[j] = ld_stream_256(pb + at * 64);
+        sa[j] = __half_as_ushort(qa[at]);
+        sb[j] = __half_as_ushort(qb[at]);
+        e[j] = *reinterpret_cast<const uint4*>(xe + at * 64);
+        o[j] = *reinterpret_cast<const uint4*>(xo + at * 64);
+        f0[j] = WHOLE || j <= last ? x0[at] : 0.f;
+        f1[j] = WHOLE || j <= last ? x1[at] : 0.f;
+    };
+    Unit un = find_unit_of_chunk(p, u, COLS, tiles, ends);
+    start(un);
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[t][i] = 0.f;
-        if (live) {
-            // the two weight rows of this lane's fragment (rows past the end repeat the last one and are not stored)
-            const int ra = min(n0 + fr, p.N - 1), rb = GATED ? p.N + ra : min(n0 + 8 + fr, p.N - 1);
-            const size_t row0 = (size_t)un.expert * (GATED ? 2 * p.N : p.N);
-            const uint8_t* wa = p.wq + (row0 + ra) * (size_t)(p.K / 2) + fq * 16;
-            const uint8_t* wb = p.wq + (row0 + rb) * (size_t)(p.K / 2) + fq * 16;
-            const __half* sa = p.ws + (row0 + ra) * (size_t)G;
-            const __half* sb = p.ws + (row0 + rb) * (size_t)G;
-            const int8_t *xe[NT], *xo[NT];                            // codes of column fr; nullptr: no such row
-            const float* cs[NT][2];                                   // scales of columns 2 fq and 2 fq + 1
-            const int* cu[NT][2];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const long long r = x_row(p, un, t * 8 + fr);
-                xe[t] = r < 0 ? nullptr : p.ae + (size_t)r * (p.K / 2) + fq * 16;
-                xo[t] = r < 0 ? nullptr : p.ao + (size_t)r * (p.K / 2) + fq * 16;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const long long c = x_row(p, un, t * 8 + fq * 2 + h);
-                    cs[t][h] = c < 0 ? nullptr : p.asc + (size_t)c * G;
-                    cu[t][h] = c < 0 ? nullptr : p.asu + (size_t)c * G;
-                }
+    for (int j = 0; j < CH; j++) load(j, G - 1 - c0 * CH);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    int buf = 0;
+    while (true) {
+        Unit nu = un;
+        const bool more = u + 1 < u1;
+        for (int c = c0; c < c1; c++) {
+            const bool ends_unit = c + 1 == c1;
+            if (!ends_unit) {
+                pa += CH * 64;
+                pb += CH * 64;
+                qa += CH;
+                qb += CH;
+                xe += CH * 64;
+                xo += CH * 64;
+                x0 += CH;
+                x1 += CH;
+            } else if (more) {
+                nu = find_unit_of_chunk(p, u + 1, COLS, tiles, ends);
+                start(nu);
             }
-#pragma unroll 2
-            for (int g = part; g < G; g += wk) {
-                const uint4 va = ld_stream_v4(wa + (size_t)g * 64), vb = ld_stream_v4(wb + (size_t)g * 64);
-                const float fa = __half2float(sa[g]), fb = __half2float(sb[g]);
+            const bool fetch = !ends_unit || more;
+            const int last = G - 1 - (ends_unit ? c0 : c + 1) * CH;
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const uint4 z = make_uint4(0, 0, 0, 0);
-                    const uint4 e = xe[t] ? *reinterpret_cast<const uint4*>(xe[t] + (size_t)g * 64) : z;
-                    const uint4 o = xo[t] ? *reinterpret_cast<const uint4*>(xo[t] + (size_t)g * 64) : z;
-                    const float s0 = cs[t][0] ? cs[t][0][g] : 0.f, s1 = cs[t][1] ? cs[t][1][g] : 0.f;
-                    const int u0q = cu[t][0] ? -8 * cu[t][0][g] : 0, u1q = cu[t][1] ? -8 * cu[t][1][g] : 0;
-                    int c[4] = {u0q, u1q, u0q, u1q};
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        mma_u8s8(c, lo_u(word(va, j)), lo_u(word(vb, j)), hi_u(word(va, j)), hi_u(word(vb, j)), word(e, j), word(o, j));
-                    acc[t][0] = fmaf((float)c[0], fa * s0, acc[t][0]);
-                    acc[t][1] = fmaf((float)c[1], fa * s1, acc[t][1]);
-                    acc[t][2] = fmaf((float)c[2], fb * s0, acc[t][2]);
-                    acc[t][3] = fmaf((float)c[3], fb * s1, acc[t][3]);
-                }
+            for (int j = 0; j < CH; j++) {
+                int d[4];
+                mma_s8_first(d, lo16(wa[j].x), lo16(wb[j].x), hi16(wa[j].x), hi16(wb[j].x), e[j].x, o[j].x);
+                mma_s8(d, lo16(wa[j].y), lo16(wb[j].y), hi16(wa[j].y), hi16(wb[j].y), e[j].y, o[j].y);
+                mma_s8(d, lo16(wa[j].z), lo16(wb[j].z), hi16(wa[j].z), hi16(wb[j].z), e[j].z, o[j].z);
+                mma_s8(d, lo16(wa[j].w), lo16(wb[j].w), hi16(wa[j].w), hi16(wb[j].w), e[j].w, o[j].w);
+                const float fa = __half2float(__ushort_as_half(sa[j])), fb = __half2float(__ushort_as_half(sb[j]));
+                acc[0] = fmaf((float)d[0], fa * f0[j], acc[0]);
+                acc[1] = fmaf((float)d[1], fa * f1[j], acc[1]);
+                acc[2] = fmaf((float)d[2], fb * f0[j], acc[2]);
+                acc[3] = fmaf((float)d[3], fb * f1[j], acc[3]);
+                if (fetch) load(j, last);
             }
         }
-        if (wk > 1) {                                                 // add the K parts, in the order of the parts
-            __syncthreads();
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+        for (int i = 0; i < 4; i++) acc[i] *= 0.0625f;
+        if (wk > 1) {                                                 // add the parts, in their order
 #pragma unroll
-                for (int i = 0; i < 4; i++) join[warp][t][i][lane] = acc[t][i];
-            __syncthreads();
-            if (part == 0) {
+            for (int i = 0; i < 4; i++) join[buf][warp][i][lane] = acc[i];
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(wk * 32) : "memory");          // (two buffers: one barrier a unit)
+            if (part == 0)
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        for (int k = 1; k < wk; k++) acc[t][i] += join[warp + k][t][i][lane];
-            }
+                for (int i = 0; i < 4; i++)
+                    for (int k = 1; k < wk; k++) acc[i] += join[buf][warp + k][i][lane];
+            buf ^= 1;
         }
-        if (live && part == 0) {
+        if (part == 0) {
+            const int n0 = un.tile * ROWS;
             const float* bias = p.bias ? p.bias + (size_t)un.expert * (GATED ? 2 * p.N : p.N) : nullptr;
             const int na = n0 + fr, nb = GATED ? p.N + na : na + 8;   // the lane's two weight rows
             const bool has_a = na < p.N, has_b = GATED ? has_a : nb < p.N;
             const float ba = bias && has_a ? bias[na] : 0.f, bb = bias && has_b ? bias[nb] : 0.f;
-            const long long end = (long long)un.first + un.count;
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const long long m = (long long)un.first + t * 8 + fq * 2;
-                float v[2] = {acc[t][0] + ba, acc[t][1] + ba}, w[2] = {acc[t][2] + bb, acc[t][3] + bb};
-                if (m >= end) continue;
+            const long long m = (long long)un.first + fq * 2, end = (long long)un.first + un.count;
+            float v[2] = {acc[0] + ba, acc[1] + ba}, w[2] = {acc[2] + bb, acc[3] + bb};
+            if (m < end) {
                 if (GATED) {
                     if (has_a) finish<2, true>(p, m, 1, end, na, v, w);
                 } else {
@@ -140,31 +176,38 @@ rows_kernel(const Params p, int wk) {
                 }
             }
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = 0.f;
+        if (!more) break;
+        un = nu;
+        u++;
     }
     pdl_launch_dependents();
 }
 
-template <int NT>
 cudaError_t run_rows(const LaunchCtx& c, const Params& p) {
-    const int cols = 8 * NT, rows = p.gated ? 8 : 16, tiles = (p.N + rows - 1) / rows, G = p.K / 128;
-    // the K dimension is split over the warps of a CTA while a warp keeps at least four groups
-    int wk = 1;
-    while (wk < kWarps && G / (wk * 2) >= 4) wk *= 2;
-    long long chunks = (p.m + cols - 1) / cols;
+    const int rows = p.gated ? 8 : 16, tiles = (p.N + rows - 1) / rows, parts = (p.K / 128 + CH - 1) / CH;
+    long long chunks = (p.m + COLS - 1) / COLS;
     if (p.offsets) chunks = p.n_exp < p.m ? chunks + p.n_exp : p.m;   // every bucket may end in a part of a chunk
-    const long long units = chunks * tiles;
-    long long grid = (units + kWarps / wk - 1) / (kWarps / wk);
-    if (grid > c.sm_count * 8LL) grid = c.sm_count * 8LL;
+    const long long units = chunks * tiles, slots = (long long)c.sm_count * kCtasPerSm * kMaxWarps;
+    // the K dimension is split over warps while all of them stay resident at once and each keeps a chunk
+    int wk = (int)(slots / units < kMaxWarps ? slots / units : kMaxWarps);
+    if (wk > parts) wk = parts;
+    if (wk < 1) wk = 1;
+    const int per_cta = kMaxWarps / wk;
+    long long grid = (units + per_cta - 1) / per_cta;
+    if (grid > c.sm_count * kCtasPerSm) grid = c.sm_count * kCtasPerSm;
     const size_t smem = p.offsets ? (size_t)p.n_exp * 4 : 0;
-    return p.gated ? launch_kernel(rows_kernel<NT, true>, dim3((unsigned)grid), dim3(kThreads), smem, c.stream, pdl_enabled(), p, wk)
-                   : launch_kernel(rows_kernel<NT, false>, dim3((unsigned)grid), dim3(kThreads), smem, c.stream, pdl_enabled(), p, wk);
+    const bool whole = p.K % 512 == 0;
+    auto kern = p.gated ? (whole ? rows_kernel<true, true> : rows_kernel<true, false>) : (whole ? rows_kernel<false, true> : rows_kernel<false, false>);
+    return launch_kernel(kern, dim3((unsigned)grid), dim3(wk * per_cta * 32), smem, c.stream, pdl_enabled(), p, wk);
 }
 
 int run(const char* kn, const LaunchCtx& c, const Params& p) {
     // rows per bucket, were all experts equally popular
     const int per = p.offsets ? p.m / (p.n_exp < p.m ? p.n_exp : p.m) : p.m;
-    if (per >= 16) return run_tiles(kn, c, p);
-    const cudaError_t e = p.m <= 8 || p.offsets ? run_rows<1>(c, p) : run_rows<2>(c, p);
+    if (per > 16) return run_tiles(kn, c, p);
+    const cudaError_t e = run_rows(c, p);
     return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
 }
 

@@ -105,7 +105,10 @@ __device__ __forceinline__ int count_units(const Params& p, int cols, int tiles,
     return carry;
 }
 
-__device__ __forceinline__ Unit find_unit(const Params& p, int u, int cols, int tiles, const int* ends) {
+// TILE_LAST: the units of a bucket walk its chunks of rows first (they share a tile of weights), otherwise its tiles first
+// (they share rows of x).
+template <bool TILE_LAST>
+__device__ __forceinline__ Unit find_unit_by(const Params& p, int u, int cols, int tiles, const int* ends) {
     Unit r;
     int lo = 0, begin = 0, end = p.m;
     if (p.offsets) {
@@ -121,11 +124,17 @@ __device__ __forceinline__ Unit find_unit(const Params& p, int u, int cols, int 
     }
     const int chunks = (end - begin + cols - 1) / cols;
     r.expert = lo;
-    r.tile = u / chunks;
-    r.first = begin + (u - r.tile * chunks) * cols;
+    const int i = TILE_LAST ? u / chunks : u / tiles, j = u - i * (TILE_LAST ? chunks : tiles);
+    r.tile = TILE_LAST ? i : j;
+    r.first = begin + (TILE_LAST ? j : i) * cols;
     r.count = min(cols, end - r.first);
     r.pad = 0;
     return r;
+}
+
+__device__ __forceinline__ Unit find_unit(const Params& p, int u, int cols, int tiles, const int* ends) { return find_unit_by<true>(p, u, cols, tiles, ends); }
+__device__ __forceinline__ Unit find_unit_of_chunk(const Params& p, int u, int cols, int tiles, const int* ends) {
+    return find_unit_by<false>(p, u, cols, tiles, ends);
 }
 
 // row of x that column c of the unit takes, or -1
