@@ -9,6 +9,8 @@
 //       ids[t, j], j < topk: the experts of the topk largest keys, descending, equal keys by ascending index;
 //       weights[t, j] = s[ids], divided by their sum when renorm is set, times scale.
 //       A logit of -inf or NaN (or such a bias) takes the expert out; a choice without a candidate is id -1, weight 0.
+//   moe_route_plan_k(logits, bias, ids, weights, bucket_rows, base, offsets, rows, ..., dtype)
+//       moe_route_k and moe_plan_k behind each other; few tokens in one launch.
 //   moe_plan_k(ids, weights, bucket_rows, base, offsets, rows, n_exp, topk)
 //       counting sort of the pairs by expert, stable by pair index: offsets[n_exp + 1] bounds the buckets,
 //       bucket_rows[slot] is the token of a slot, base[t, j] the slot of a pair.  A pair whose id is out of range or
@@ -33,8 +35,12 @@ struct RouteParams {
     int* ids;
     float* weights;
     int rows, n_exp, topk, n_group, topk_group, group_top, group_size;
-    bool sigmoid, renorm;
+    int group_lanes;           // lanes to a group when that is a power of two of whole lanes, else 0
+    int dtype;
+    bool sigmoid, renorm, vector;
     float scale;
+    // moe_route_plan_k
+    int *bucket_rows, *base, *offsets, *hist;
 };
 
 __device__ __forceinline__ float logit_at(const float* p, size_t i) { return p[i]; }
@@ -54,262 +60,620 @@ __device__ __forceinline__ float key_value(uint32_t u) { return u ? __uint_as_fl
 __device__ __forceinline__ double key_value(uint64_t u) {
     return u ? __longlong_as_double((long long)(u & 0x8000000000000000ull ? u ^ 0x8000000000000000ull : ~u)) : -INFINITY;
 }
-__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ uint64_t warp_max(uint64_t v) {
     const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
     const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
     return (uint64_t)hi << 32 | lo;
 }
 
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
-__device__ __forceinline__ double warp_sum(double v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+__device__ __forceinline__ float exp2f_approx(float x) {
+    float d;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+    return d;
 }
-using fm::warp_sum;
+__device__ __forceinline__ float rcp_approx(float x) {
+    float d;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+    return d;
+}
 
-template <typename R> struct KeyOf;
-template <> struct KeyOf<float> { typedef uint32_t type; };
-template <> struct KeyOf<double> { typedef uint64_t type; };
-
-// Two fp32 keys of at most this magnitude are told apart for certain when they are this far from each other: exp and
-// the division are within 2^-22, a sum of up to 1024 scores (32 in turn, then five halvings) within 37 * 2^-24 of their
-// values, which are at most 1; adding the bias rounds by at most 2^-24 of the key.
+// Two fp32 keys of at most this magnitude are told apart for certain when they are this far from each other: the score is
+// at most 1, its exp within 2^-22 and, the argument x log2(e) being rounded, within |x| 2^-24, of which the score sees at
+// most x exp(-x) <= 0.37; the reciprocal is within 2^-23, a sum of up to 1024 scores (32 in turn, then five halvings) within
+// 37 * 2^-24; adding the bias rounds by at most 2^-24 of the key.  2^-17 is over twice the sum of these.
 __device__ __forceinline__ float resolution(float most) { return 7.6293945e-6f + 2.3841858e-7f * most; }
 
-// s of the lane's experts (expert i * 32 + lane) in precision R
-template <typename R, int VPL>
-__device__ __forceinline__ void scores(const float (&x)[VPL], bool sigmoid, R (&s)[VPL]) {
-    if (sigmoid) {
-#pragma unroll
-        for (int i = 0; i < VPL; i++) s[i] = R(1) / (R(1) + exp_of(-(R)x[i]));
-        return;
-    }
+// ---- the decision in fp64: lane's experts lane * VPL + i, plain loops; taken for the few tokens that fp32 cannot decide
+template <int VPL>
+__device__ __noinline__ int decide64(const RouteParams& p, const float* __restrict__ xs, double* stage) {
+    const int lane = threadIdx.x & 31;
+    double s[VPL];
+    float x[VPL];
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < VPL; i++) m = fmaxf(m, x[i]);
+    for (int i = 0; i < VPL; i++) {
+        x[i] = xs[i];
+        m = fmaxf(m, x[i]);
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    R z = 0;
+    double z = 0.0;
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
-        s[i] = x[i] == m ? R(1) : x[i] > -INFINITY ? exp_of((R)x[i] - (R)m) : R(0);   // (an infinite maximum is its own score)
-        if (!(x[i] > -INFINITY)) s[i] = 0;
-        z += s[i];
-    }
-    z = warp_sum(z);
-#pragma unroll
-    for (int i = 0; i < VPL; i++) s[i] = s[i] / z;
-}
-
-// Takes the experts of all but the best groups out of the keys.  `s`: the values that make a group's worth.  Returns
-// the distance between the worst group kept and the best one dropped (for the caller's decision whether R resolves it).
-template <typename R, int VPL>
-__device__ __forceinline__ R limit_groups(const RouteParams& p, typename KeyOf<R>::type (&key)[VPL], const R (&s)[VPL], R* stage) {
-    typedef typename KeyOf<R>::type Key;
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < VPL; i++)
-        if (i * 32 + lane < p.n_exp) stage[i * 32 + lane] = key[i] ? s[i] : -INFINITY;
-    __syncwarp();
-    R worth = -INFINITY;
-    if (lane < p.n_group) {
-        R a = -INFINITY, b = -INFINITY;
-        int j = lane % p.group_size;                                  // (lanes start apart: fewer bank conflicts)
-        for (int k = 0; k < p.group_size; k++) {
-            const R v = stage[lane * p.group_size + j];
-            if (v > a) { b = a; a = v; }
-            else if (v > b) b = v;
-            if (++j == p.group_size) j = 0;
+        if (p.sigmoid) s[i] = 1.0 / (1.0 + exp(-(double)x[i]));
+        else {
+            s[i] = !(x[i] > -INFINITY) ? 0.0 : x[i] == m ? 1.0 : exp((double)x[i] - (double)m);
+            z += s[i];
         }
-        worth = p.group_top == 2 && p.group_size > 1 ? (b > -INFINITY ? a + b : a) : a;
     }
-    __syncwarp();
-    Key w = ordered(worth);
-    uint32_t kept = 0;
-    R last = 0, next = -INFINITY;
-    for (int k = 0; k <= p.topk_group && k < p.n_group; k++) {
-        const Key best = warp_max(w);
-        if (k == p.topk_group) { next = key_value(best); break; }
-        if (best == 0) { last = INFINITY; break; }                    // the other groups are empty
-        const int g = __ffs(__ballot_sync(0xffffffffu, w == best)) - 1;
-        kept |= 1u << g;
-        last = key_value(best);
-        if (lane == g) w = 0;
-    }
+    if (!p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < VPL; i++)
-        if (!((kept >> ((i * 32 + lane) / p.group_size & 31)) & 1u)) key[i] = 0;
-    return last - next;
-}
-
-// The topk experts of the token in order: lane j returns the j-th (-1: none).  `near` becomes true when two keys that
-// follow each other are closer than fp32 tells apart and do not come from equal inputs (checked for R = float only).
-template <typename R, int VPL>
-__device__ __forceinline__ int pick(const RouteParams& p, typename KeyOf<R>::type (&key)[VPL], const float (&x)[VPL], bool check, bool& near) {
-    typedef typename KeyOf<R>::type Key;
-    const int lane = threadIdx.x & 31;
+        for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    }
+    uint64_t key[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; i++) {
+        const int e = lane * VPL + i;
+        if (!p.sigmoid) s[i] = s[i] / z;
+        if (p.bias && e < p.n_exp) s[i] += (double)p.bias[e];
+        key[i] = x[i] > -INFINITY ? ordered(p.bias ? s[i] : (double)x[i]) : 0ull;
+    }
+    if (p.n_group > 1) {
+        const bool by_key = !p.bias && p.group_top == 1;              // (the order of the logits is that of the scores)
+#pragma unroll
+        for (int i = 0; i < VPL; i++)
+            if (lane * VPL + i < p.n_exp) stage[lane * VPL + i] = !key[i] ? -INFINITY : by_key ? (double)x[i] : s[i];
+        __syncwarp();
+        uint64_t w = 0;
+        if (lane < p.n_group) {
+            double a = -INFINITY, b = -INFINITY;
+            for (int k = 0; k < p.group_size; k++) {
+                const double v = stage[lane * p.group_size + k];
+                if (v > a) { b = a; a = v; }
+                else if (v > b) b = v;
+            }
+            w = ordered(p.group_top == 2 && b > -INFINITY ? a + b : a);
+        }
+        __syncwarp();
+        uint32_t kept = 0;
+        for (int k = 0; k < p.topk_group; k++) {
+            const uint64_t best = warp_max(w);
+            if (best == 0) break;
+            const int g = __ffs(__ballot_sync(0xffffffffu, w == best)) - 1;
+            kept |= 1u << g;
+            if (lane == g) w = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < VPL; i++) {
+            const int e = lane * VPL + i;
+            if (e < p.n_exp && !((kept >> (e / p.group_size)) & 1u)) key[i] = 0;
+        }
+    }
     int mine = -1;
-    float px = 0.f, pb = 0.f;
-    R prev = INFINITY;
-    for (int j = 0; j < p.topk + (check ? 1 : 0); j++) {
-        Key best = 0;
-        int at = 0;
+    for (int j = 0; j < p.topk; j++) {
+        uint64_t best = 0;
 #pragma unroll
-        for (int i = 0; i < VPL; i++)
-            if (key[i] > best) { best = key[i]; at = i; }
-        const Key top = warp_max(best);
+        for (int i = 0; i < VPL; i++) best = key[i] > best ? key[i] : best;
+        const uint64_t top = warp_max(best);
         if (top == 0) break;
-        const int e = (int)__reduce_min_sync(0xffffffffu, best == top ? (uint32_t)(at * 32 + lane) : 0xffffffffu);
-        float ex = 0.f;
+        const int from = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+        int at = 0;
+        if (lane == from) {
 #pragma unroll
-        for (int i = 0; i < VPL; i++)
-            if (i * 32 + lane == e) { key[i] = 0; ex = x[i]; }
-        if (check) {
-            ex = __shfl_sync(0xffffffffu, ex, e & 31);
-            const float eb = p.bias[e];
-            const R v = key_value(top);
-            if (j > 0 && !(prev - v > resolution((float)fmaxf(fabsf((float)v), fabsf((float)prev)))) && !(ex == px && eb == pb)) near = true;
-            prev = v;
-            px = ex;
-            pb = eb;
+            for (int i = VPL - 1; i >= 0; i--)
+                if (key[i] == top) at = i;
+#pragma unroll
+            for (int i = 0; i < VPL; i++)
+                if (i == at) key[i] = 0;
         }
-        if (j < p.topk && lane == j) mine = e;
+        at = __shfl_sync(0xffffffffu, at, from);
+        if (lane == j) mine = from * VPL + at;
     }
     return mine;
 }
 
-// One warp per token.  With a bias the keys are rounded sums: they are formed in fp32 first, and a token where two
-// keys (or the last group kept and the first one dropped) lie within the error of fp32 is decided again in fp64, so
-// that the choice is that of the exact keys at fp32's cost.
-template <typename T, int VPL>
-__global__ void __launch_bounds__(128)
-route_kernel(const RouteParams p) {
-    extern __shared__ double stage_all[];
-    pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.x * 4 + warp;
-    if (row >= p.rows) return;
-    double* stage = stage_all + (size_t)warp * p.n_exp;
-    const T* in = reinterpret_cast<const T*>(p.logits) + (size_t)row * p.n_exp;
-    float x[VPL];
+// ---- the decision in fp32
+// exp and 1 / x to 2^-21 at least: good enough to order by (see `resolution`), not for the weights
+__device__ __forceinline__ float fast_exp(float x) { return exp2f_approx(x * 1.4426950f); }
+
+// Sorts the lane's keys, descending, equal keys by ascending position; `at` holds the positions, four bits each.
+template <int VPL>
+__device__ __forceinline__ void sort_lane(uint32_t (&k)[VPL], uint32_t& order) {
+    uint32_t at[VPL];
 #pragma unroll
-    for (int i = 0; i < VPL; i++) {
-        const int e = i * 32 + lane;
-        x[i] = e < p.n_exp ? logit_at(in, e) : -INFINITY;
-        if (!(x[i] > -INFINITY)) x[i] = -INFINITY;                    // NaN: never chosen
-    }
-    float s[VPL];
-    scores<float, VPL>(x, p.sigmoid, s);
-    uint32_t key[VPL];
-    int mine;
-    if (!p.bias) {
+    for (int i = 0; i < VPL; i++) at[i] = i;
+    // Batcher's odd-even merge sort (1968)
 #pragma unroll
-        for (int i = 0; i < VPL; i++) key[i] = ordered(x[i]);
-        bool near = false;
-        if (p.n_group > 1 && p.group_top == 1) limit_groups<float, VPL>(p, key, x, reinterpret_cast<float*>(stage));
-        else if (p.n_group > 1) {
-            const float gap = limit_groups<float, VPL>(p, key, s, reinterpret_cast<float*>(stage));
-            near = !(gap > 2.f * resolution(1.f));
+    for (int p = 1; p < VPL; p <<= 1)
+#pragma unroll
+        for (int q = p; q >= 1; q >>= 1)
+#pragma unroll
+            for (int j = q % p; j + q < VPL; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; i++)
+                    if (i + j + q < VPL && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const int a = i + j, b = i + j + q;
+                        const bool swap = k[b] > k[a] || (k[b] == k[a] && at[b] < at[a]);
+                        const uint32_t ka = k[a], ia = at[a];
+                        k[a] = swap ? k[b] : ka;
+                        at[a] = swap ? at[b] : ia;
+                        k[b] = swap ? ka : k[b];
+                        at[b] = swap ? ia : at[b];
+                    }
+    order = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; i++) order |= at[i] << (4 * (i & 7));
+}
+
+// The topk largest keys of the warp in order, as positions lane * VPL + i, and (with `more`) the key after them: lane j gets
+// the j-th position (-1: none) and key.  Keys of up to eight a lane come sorted (`order`: their positions).
+template <int VPL>
+__device__ __forceinline__ int pick(int rounds, uint32_t (&key)[VPL], uint32_t order, uint32_t& kept) {
+    const int lane = threadIdx.x & 31;
+    int mine = -1;
+    kept = 0;
+    for (int j = 0; j < rounds; j++) {
+        uint32_t best = key[0];
+        if (VPL > 8) {
+#pragma unroll
+            for (int i = 1; i < VPL; i++) best = max(best, key[i]);
         }
-        if (near) {
-            double sd[VPL];
-            uint64_t kd[VPL];
-            scores<double, VPL>(x, p.sigmoid, sd);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        if (top == 0) break;
+        const int from = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+        int at = (int)(order & 15u);
+        const bool hit = lane == from;
+        if (VPL <= 8) {                                               // sorted: the next one moves up
 #pragma unroll
-            for (int i = 0; i < VPL; i++) kd[i] = ordered((double)x[i]);
-            limit_groups<double, VPL>(p, kd, sd, stage);
+            for (int i = 0; i + 1 < VPL; i++) key[i] = hit ? key[i + 1] : key[i];
+            key[VPL - 1] = hit ? 0u : key[VPL - 1];
+            order = hit ? order >> 4 : order;
+        } else {
+            at = 0;
 #pragma unroll
-            for (int i = 0; i < VPL; i++) key[i] = kd[i] ? ordered(x[i]) : 0u;
-        }
-        mine = pick<float, VPL>(p, key, x, false, near);
-    } else {
-        float v[VPL];
-#pragma unroll
-        for (int i = 0; i < VPL; i++) {
-            const int e = i * 32 + lane;
-            v[i] = x[i] > -INFINITY ? s[i] + p.bias[e] : -INFINITY;
-            key[i] = ordered(v[i]);
-        }
-        bool near = false;
-        if (p.n_group > 1) {
-            float most = 0.f;                                         // the largest finite key: what fp32 resolves
+            for (int i = VPL - 1; i >= 0; i--)
+                if (key[i] == top) at = i;
 #pragma unroll
             for (int i = 0; i < VPL; i++)
-                if (key[i]) most = fmaxf(most, fabsf(v[i]));
-#pragma unroll
-            for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            const float gap = limit_groups<float, VPL>(p, key, v, reinterpret_cast<float*>(stage));
-            near = !(gap > 2.f * resolution(most));                   // (a group's worth is a sum of two)
+                if (hit && i == at) key[i] = 0;
         }
-        if (!near) mine = pick<float, VPL>(p, key, x, true, near);
-        if (near) {
-            double vd[VPL];
-            uint64_t kd[VPL];
-            scores<double, VPL>(x, p.sigmoid, vd);
-#pragma unroll
-            for (int i = 0; i < VPL; i++) {
-                vd[i] = x[i] > -INFINITY ? vd[i] + (double)p.bias[i * 32 + lane] : -INFINITY;
-                kd[i] = ordered(vd[i]);
-            }
-            if (p.n_group > 1) limit_groups<double, VPL>(p, kd, vd, stage);
-            mine = pick<double, VPL>(p, kd, x, false, near);
+        const int e = from * VPL + __shfl_sync(0xffffffffu, at, from);
+        if (lane == j) {
+            mine = e;
+            kept = top;
         }
     }
-    // the scores of the chosen, from the lanes that hold them
-    float w = 0.f;
-    for (int j = 0; j < p.topk; j++) {
-        const int e = __shfl_sync(0xffffffffu, mine, j);
-        float v = 0.f;
+    return mine;
+}
+
+// Which groups stay, as a mask.  a, b: the two best of the lane's group (group_lanes > 0) or of group `lane`.  gap: the distance
+// between the worst group kept and the best one dropped.
+__device__ __forceinline__ uint32_t best_groups(const RouteParams& p, float a, float b, float& gap) {
+    const int lane = threadIdx.x & 31, lanes = p.group_lanes;
+    for (int o = 1; o < lanes; o <<= 1) {
+        const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+        b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+        a = fmaxf(a, oa);
+    }
+    const int group = lanes > 0 ? lane / lanes : lane;
+    const bool speaks = group < p.n_group && (lanes <= 1 || lane % lanes == 0);          // one lane of a group speaks for it
+    uint32_t w = speaks ? ordered(p.group_top == 2 && b > -INFINITY ? a + b : a) : 0u;
+    uint32_t kept = 0;
+    float last = INFINITY, next = -INFINITY;
+    for (int k = 0; k <= p.topk_group; k++) {
+        const uint32_t best = __reduce_max_sync(0xffffffffu, w);
+        if (k == p.topk_group) {
+            next = key_value(best);
+            break;
+        }
+        if (best == 0) break;                                         // the other groups are empty
+        const int from = __ffs(__ballot_sync(0xffffffffu, w == best)) - 1;
+        kept |= 1u << (lanes > 0 ? from / lanes : from);
+        last = key_value(best);
+        if (lane == from) w = 0;
+    }
+    gap = last - next;
+    return kept;
+}
+
+template <int VPL, typename T>
+__device__ __forceinline__ void load_logits(const RouteParams& p, size_t row, float (&x)[VPL]) {
+    const int lane = threadIdx.x & 31;
+    const T* in = reinterpret_cast<const T*>(p.logits) + row * p.n_exp + lane * VPL;
+    constexpr int PER = 16 / (int)sizeof(T);
+    if (VPL % PER == 0 && p.n_exp == 32 * VPL && p.vector) {          // whole 16-byte words
+#pragma unroll
+        for (int i = 0; i < VPL; i += PER) {
+            const uint4 w = *reinterpret_cast<const uint4*>(in + i);
+            const T* t = reinterpret_cast<const T*>(&w);
+#pragma unroll
+            for (int k = 0; k < PER; k++) x[(i + k) % VPL] = logit_at(t, k);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; i++) x[i] = lane * VPL + i < p.n_exp ? logit_at(in, i) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; i++)
+        if (!(x[i] > -INFINITY)) x[i] = -INFINITY;                    // NaN: never chosen
+}
+
+// One token: lane j < topk gets its j-th expert and weight.  Keys are formed and ordered in fp32; a token where two that
+// matter lie within the error of fp32 is decided again in fp64, so that the choice is that of the exact keys at fp32's cost.
+// bias: the lane's, `most`: the largest magnitude that a finite key can have.
+template <int VPL, typename T>
+__device__ __forceinline__ void route_token(const RouteParams& p, size_t row, const float (&bias)[VPL], float most, double* stage, int& id, float& weight) {
+    const int lane = threadIdx.x & 31;
+    float x[VPL], s[VPL];                                             // logits; scores to order by
+    load_logits<VPL, T>(p, row, x);
+    float m = 0.f, z = 1.f;
+    const bool by_score = !p.bias && p.n_group > 1 && p.group_top == 2, need = p.bias || by_score;
+    if (!p.sigmoid) {
+        m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VPL; i++) m = fmaxf(m, x[i]);
+        m = key_value(__reduce_max_sync(0xffffffffu, ordered(m)));
+        if (need || !p.renorm) {
+            z = 0.f;
+#pragma unroll
+            for (int i = 0; i < VPL; i++) {                           // (an infinite maximum is its own score)
+                s[i] = !(x[i] > -INFINITY) ? 0.f : x[i] == m ? 1.f : p.renorm ? fast_exp(x[i] - m) : expf(x[i] - m);
+                z += s[i];
+            }
+            z = warp_sum(z);
+            const float r = 1.f / z;
+#pragma unroll
+            for (int i = 0; i < VPL; i++) s[i] *= r;
+        }
+    } else if (need) {
+#pragma unroll
+        for (int i = 0; i < VPL; i++) s[i] = rcp_approx(1.f + fast_exp(-x[i]));
+    }
+    uint32_t key[VPL], order = 0, kept = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; i++) key[i] = ordered(!p.bias ? x[i] : x[i] > -INFINITY ? s[i] + bias[i] : -INFINITY);
+    bool near = false;
+    float a = -INFINITY, b = -INFINITY;                               // the two best of the lane
+    if (by_score) {
+#pragma unroll
+        for (int i = 0; i < VPL; i++) {
+            const float t = key[i] ? s[i] : -INFINITY;
+            b = fmaxf(b, fminf(a, t));
+            a = fmaxf(a, t);
+        }
+    }
+    if (p.n_group > 1 && p.group_lanes == 0) {                        // groups that do not end with lanes
+        float* list = reinterpret_cast<float*>(stage);
 #pragma unroll
         for (int i = 0; i < VPL; i++)
-            if (i * 32 + lane == e) v = s[i];
-        v = __shfl_sync(0xffffffffu, v, e & 31);
-        if (lane == j && e >= 0) w = v;
+            if (lane * VPL + i < p.n_exp) list[lane * VPL + i] = by_score && key[i] ? s[i] : key_value(key[i]);
+        __syncwarp();
+        a = b = -INFINITY;
+        if (lane < p.n_group)
+            for (int k = 0; k < p.group_size; k++) {
+                const float t = list[lane * p.group_size + k];
+                b = fmaxf(b, fminf(a, t));
+                a = fmaxf(a, t);
+            }
+        __syncwarp();
+        float gap;
+        const uint32_t groups = best_groups(p, a, b, gap);
+        near = need && !(gap > 2.f * resolution(most));               // (a group's worth is a sum of two)
+#pragma unroll
+        for (int i = 0; i < VPL; i++) {
+            const int e = lane * VPL + i;
+            if (e < p.n_exp && !((groups >> (e / p.group_size)) & 1u)) key[i] = 0;
+        }
+    }
+    if (VPL <= 8) sort_lane<VPL>(key, order);
+    if (p.n_group > 1 && p.group_lanes > 0) {
+        if (!by_score) {
+            if (VPL <= 8) {
+                a = key_value(key[0]);
+                if (VPL > 1) b = key_value(key[VPL > 1 ? 1 : 0]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VPL; i++) {
+                    const float t = key_value(key[i]);
+                    b = fmaxf(b, fminf(a, t));
+                    a = fmaxf(a, t);
+                }
+            }
+        }
+        float gap;
+        const uint32_t groups = best_groups(p, a, b, gap);
+        near = need && !(gap > 2.f * resolution(most));
+        if (!((groups >> ((lane / p.group_lanes) & 31)) & 1u)) {
+#pragma unroll
+            for (int i = 0; i < VPL; i++) key[i] = 0;
+        }
+    }
+    id = pick<VPL>(min(p.topk + (p.bias ? 1 : 0), 32), key, order, kept);
+    if (p.bias) {
+        // (with 32 choices the key after them has no lane: two of all are then compared below 32 only, and fp64 decides)
+        const float v = key_value(kept), prev = __shfl_up_sync(0xffffffffu, v, 1);
+        const int before = __shfl_up_sync(0xffffffffu, id, 1);
+        bool close = lane > 0 && lane <= p.topk && id >= 0 && !(prev - v > resolution(fmaxf(fabsf(v), fabsf(prev))));
+        if (close) {                                                  // equal inputs are equal keys: the order of the index is right
+            const T* in = reinterpret_cast<const T*>(p.logits) + row * p.n_exp;
+            close = !(logit_at(in, id) == logit_at(in, before) && p.bias[id] == p.bias[before]);
+        }
+        near = near || p.topk == 32 || __any_sync(0xffffffffu, close);
+    }
+    if (near) {
+        float copy[VPL];                                              // (an array whose address is taken lives in memory)
+#pragma unroll
+        for (int i = 0; i < VPL; i++) copy[i] = x[i];
+        id = decide64<VPL>(p, copy, stage);
+    }
+    if (lane >= p.topk) id = -1;
+    // the weight of the lane's choice, from its logit
+    float w = 0.f;
+    if (id >= 0) {
+        const float c = logit_at(reinterpret_cast<const T*>(p.logits), row * p.n_exp + id);
+        if (p.sigmoid) w = __frcp_rn(1.f + expf(-c));
+        else w = c == m ? 1.f : expf(c - m);
+        if (!p.sigmoid && !p.renorm) w = __fdiv_rn(w, z);
     }
     if (p.renorm) {
-        const float sum = warp_sum(lane < p.topk ? w : 0.f);
-        w = sum > 0.f ? w / sum : 0.f;
+        const float sum = warp_sum(w);
+        w = sum > 0.f ? __fdiv_rn(w, sum) : 0.f;
     }
-    if (lane < p.topk) {
-        p.ids[(size_t)row * p.topk + lane] = mine;
-        p.weights[(size_t)row * p.topk + lane] = w * p.scale;
+    weight = w * p.scale;
+}
+
+// ------------------------------------------------------------------------------------------------------ the plan
+// The slot of a pair is
+//   (pairs of smaller experts) + (pairs of its expert in earlier blocks, warps, batches and lanes),
+// so the order is that of the pair indices whatever the scheduling: no atomic decides a position.
+constexpr int kThreads = 512;                       // of the counting kernel
+
+__device__ __forceinline__ int pair_expert(int id, float w, int n_exp) { return id >= 0 && id < n_exp && w != 0.f ? id : -1; }
+
+// Exclusive scan of total[0 .. n) into first[0 .. n); returns the sum.  All threads call it; total and first may be one.
+__device__ __forceinline__ int block_scan(const int* total, int* first, int n, int* part) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    int carry = 0;
+    for (int e0 = 0; e0 < n; e0 += blockDim.x) {
+        const int e = e0 + (int)threadIdx.x, v = e < n ? total[e] : 0;
+        int inc = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += t;
+        }
+        __syncthreads();
+        if (lane == 31) part[warp] = inc;
+        __syncthreads();
+        int lower = carry;
+        for (int k = 0; k < warps; k++) {
+            if (k < warp) lower += part[k];
+            carry += part[k];
+        }
+        if (e < n) first[e] = lower + inc - v;
+    }
+    __syncthreads();
+    return carry;
+}
+
+// Places the pairs [lo, hi) of this block.  first[e]: the slot of its first pair of expert e; cnt: [warps][n_exp].
+__device__ __forceinline__ void place_pairs(const int* ids, float* w, int* bucket_rows, int* base, int lo, int hi, int n_exp, int topk, const int* first,
+                                            int* cnt) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int per = ((hi - lo + warps - 1) / warps + 31) & ~31, i0 = lo + warp * per, i1 = min(i0 + per, hi);
+    int* mine = cnt + warp * n_exp;
+    for (int e = lane; e < n_exp; e += 32) mine[e] = 0;
+    __syncwarp();
+    for (int i = i0 + lane; i < i1; i += 32) {
+        const int e = pair_expert(__ldcg(ids + i), __ldcg(w + i), n_exp);
+        if (e >= 0) atomicAdd(&mine[e], 1);                           // (integers: the order does not matter)
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < n_exp; e += blockDim.x) {
+        int at = first[e];
+        for (int k = 0; k < warps; k++) {
+            const int h = cnt[k * n_exp + e];
+            cnt[k * n_exp + e] = at;
+            at += h;
+        }
+    }
+    __syncthreads();
+    for (int j0 = i0; j0 < i1; j0 += 32) {
+        const int i = j0 + lane;
+        const int e = i < i1 ? pair_expert(__ldcg(ids + i), __ldcg(w + i), n_exp) : -1;
+        const uint32_t peers = __match_any_sync(0xffffffffu, e);
+        const int rank = __popc(peers & ((1u << lane) - 1u));
+        const int slot = e >= 0 ? mine[e] + rank : 0;
+        __syncwarp();
+        if (e >= 0 && rank == 0) mine[e] += __popc(peers);
+        __syncwarp();
+        if (i < i1) {
+            base[i] = slot;
+            if (e >= 0) bucket_rows[slot] = i / topk;
+            else w[i] = 0.f;
+        }
+    }
+}
+
+__device__ unsigned g_blocks_done;                   // blocks of a fused launch that have finished; back at 0 when it ends
+
+// Block b routes the tokens [b * tokens, (b + 1) * tokens), a warp a token at a time.  With a plan: few pairs are placed by
+// the block that finishes last (fuse), otherwise every block counts its pairs of each expert for plan_place_kernel.
+template <int VPL, typename T>
+__global__ void __launch_bounds__(1024, 1)
+route_kernel(const RouteParams p, int tokens, bool fuse) {
+    extern __shared__ double dyn[];                                   // [warps][n_exp] where there are groups; then ints
+    __shared__ int next, part[32];
+    __shared__ bool last;
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    double* stage = dyn + (p.n_group > 1 ? (size_t)warp * p.n_exp : 0);
+    int* count = reinterpret_cast<int*>(dyn + (p.n_group > 1 ? (size_t)warps * p.n_exp : 0));
+    if (p.hist)
+        for (int e = threadIdx.x; e < p.n_exp; e += blockDim.x) count[e] = 0;
+    if (threadIdx.x == 0) next = warps;
+    float bias[VPL], most = 1.f;
+#pragma unroll
+    for (int i = 0; i < VPL; i++) {
+        const int e = lane * VPL + i;
+        bias[i] = p.bias && e < p.n_exp ? p.bias[e] : 0.f;
+        if (fabsf(bias[i]) < INFINITY) most = fmaxf(most, 1.f + fabsf(bias[i]));
+    }
+    if (p.bias) most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+    __syncthreads();
+    const int row0 = blockIdx.x * tokens, rows = min(tokens, p.rows - row0);
+    for (int t = warp; t < rows;) {                                   // (whichever warp is free takes the next token)
+        const size_t row = (size_t)row0 + t;
+        int id;
+        float w;
+        route_token<VPL, T>(p, row, bias, most, stage, id, w);
+        if (lane < p.topk) {
+            p.ids[row * p.topk + lane] = id;
+            p.weights[row * p.topk + lane] = w;
+            if (p.hist && pair_expert(id, w, p.n_exp) >= 0) atomicAdd(&count[id], 1);
+        }
+        if (lane == 0) t = atomicAdd(&next, 1);
+        t = __shfl_sync(0xffffffffu, t, 0);
+    }
+    if (p.hist) {
+        __syncthreads();
+        for (int e = threadIdx.x; e < p.n_exp; e += blockDim.x) p.hist[(size_t)blockIdx.x * p.n_exp + e] = count[e];
+    }
+    if (fuse) {
+        if (gridDim.x > 1) {
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) last = atomicInc(&g_blocks_done, gridDim.x - 1) == gridDim.x - 1;
+            __syncthreads();
+            if (!last) return;
+            __threadfence();
+        } else {
+            __syncthreads();
+        }
+        const int pairs = p.rows * p.topk;
+        int* total = count;                                           // [n_exp], then the warps' counts
+        int* cnt = count + p.n_exp;
+        for (int e = threadIdx.x; e < p.n_exp; e += blockDim.x) total[e] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+            const int e = pair_expert(__ldcg(p.ids + i), __ldcg(p.weights + i), p.n_exp);
+            if (e >= 0) atomicAdd(&total[e], 1);
+        }
+        __syncthreads();
+        const int sum = block_scan(total, total, p.n_exp, part);
+        for (int e = threadIdx.x; e < p.n_exp; e += blockDim.x) p.offsets[e] = total[e];
+        if (threadIdx.x == 0) p.offsets[p.n_exp] = sum;
+        place_pairs(p.ids, p.weights, p.bucket_rows, p.base, 0, pairs, p.n_exp, p.topk, total, cnt);
     }
     pdl_launch_dependents();
 }
 
-template <typename T>
-cudaError_t run_route(const LaunchCtx& c, const RouteParams& p) {
-    const dim3 grid((unsigned)((p.rows + 3) / 4)), block(128);
-    const size_t smem = p.n_group > 1 ? (size_t)4 * p.n_exp * 8 : 0;
-    const int vpl = (p.n_exp + 31) / 32;
-#define FM_ROUTE(V) return launch_kernel(route_kernel<T, V>, grid, block, smem, c.stream, pdl_enabled(), p)
-    if (vpl <= 1) FM_ROUTE(1);
-    if (vpl <= 2) FM_ROUTE(2);
-    if (vpl <= 4) FM_ROUTE(4);
-    if (vpl <= 8) FM_ROUTE(8);
-    if (vpl <= 16) FM_ROUTE(16);
-    FM_ROUTE(32);
-#undef FM_ROUTE
+// hist[block][n_exp] of pairs that are given
+__global__ void __launch_bounds__(kThreads)
+plan_count_kernel(const int* __restrict__ ids, const float* __restrict__ w, int* __restrict__ hist, int pairs, int n_exp, int per_block) {
+    extern __shared__ int count[];
+    pdl_wait();
+    for (int e = threadIdx.x; e < n_exp; e += kThreads) count[e] = 0;
+    __syncthreads();
+    const int lo = blockIdx.x * per_block, hi = min(lo + per_block, pairs);
+    for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
+        const int e = pair_expert(ids[i], w[i], n_exp);
+        if (e >= 0) atomicAdd(&count[e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < n_exp; e += kThreads) hist[(size_t)blockIdx.x * n_exp + e] = count[e];
+    pdl_launch_dependents();
 }
 
-int launch_route(const LaunchCtx& c, const uint64_t* a) {
-    const char* kn = "moe_route_k";
-    RouteParams p;
-    p.logits = arg_ptr<const void>(a[0]);
-    p.bias = arg_ptr<const float>(a[1]);
-    p.ids = arg_ptr<int>(a[2]);
-    p.weights = arg_ptr<float>(a[3]);
-    p.rows = arg_i32(a[4]);
-    p.n_exp = arg_i32(a[5]);
-    p.topk = arg_i32(a[6]);
-    p.n_group = arg_i32(a[7]);
-    p.topk_group = arg_i32(a[8]);
-    p.group_top = arg_i32(a[9]);
-    const int score = arg_i32(a[10]), renorm = arg_i32(a[11]), dtype = arg_i32(a[13]);
-    p.scale = arg_f32(a[12]);
+// Every block adds up the counts of all blocks (blockDim / n_exp threads to an expert) and places its own pairs.
+__global__ void __launch_bounds__(1024)
+plan_place_kernel(const int* __restrict__ ids, float* __restrict__ w, int* __restrict__ bucket_rows, int* __restrict__ base,
+                  int* __restrict__ offsets, const int* __restrict__ hist, int pairs, int n_exp, int topk, int per_block) {
+    extern __shared__ int sm[];
+    int* total = sm;                                                  // [n_exp]
+    int* first = sm + n_exp;                                          // [n_exp] first the pairs of earlier blocks
+    int* cnt = sm + 2 * n_exp;                                        // [warps][n_exp]
+    __shared__ int part[32];
+    pdl_wait();
+    for (int e = threadIdx.x; e < 2 * n_exp; e += blockDim.x) sm[e] = 0;
+    __syncthreads();
+    const int split = max((int)blockDim.x / n_exp, 1), blocks = gridDim.x;
+    for (int i = threadIdx.x; i < n_exp * split; i += blockDim.x) {
+        const int e = i % n_exp, s = i / n_exp;
+        int all = 0, before = 0;
+#pragma unroll 16
+        for (int b = s; b < blocks; b += split) {
+            const int h = __ldg(hist + (size_t)b * n_exp + e);
+            all += h;
+            if (b < (int)blockIdx.x) before += h;
+        }
+        if (all) {
+            atomicAdd(&total[e], all);
+            if (before) atomicAdd(&first[e], before);
+        }
+    }
+    __syncthreads();
+    const int sum = block_scan(total, total, n_exp, part);
+    for (int e = threadIdx.x; e < n_exp; e += blockDim.x) {
+        if (blockIdx.x == 0) offsets[e] = total[e];
+        first[e] += total[e];
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) offsets[n_exp] = sum;
+    __syncthreads();
+    const int lo = blockIdx.x * per_block;
+    place_pairs(ids, w, bucket_rows, base, lo, min(lo + per_block, pairs), n_exp, topk, first, cnt);
+    pdl_launch_dependents();
+}
+
+// ------------------------------------------------------------------------------------------------------- host side
+constexpr int kFusePairs = 4096;                    // placed by one block: 1.6 us for 384 pairs, a launch costs about as much
+constexpr int kFuseExperts = 256;
+
+template <typename T>
+cudaError_t run_route(const LaunchCtx& c, const RouteParams& p, int blocks, int tokens, bool fuse) {
+    int warps = tokens < 32 ? tokens : 32;
+    if (fuse && warps < 8) warps = 8;                                 // (they place the pairs)
+    const size_t smem = (p.n_group > 1 ? (size_t)warps * p.n_exp * 8 : 0) + (p.hist ? (size_t)p.n_exp * 4 : 0) + (fuse ? (size_t)p.n_exp * 4 * (1 + warps) : 0);
+    const int vpl = (p.n_exp + 31) / 32;
+    auto kern = vpl <= 1   ? route_kernel<1, T>
+                : vpl <= 2 ? route_kernel<2, T>
+                : vpl <= 4 ? route_kernel<4, T>
+                : vpl <= 8 ? route_kernel<8, T>
+                : vpl <= 16 ? route_kernel<16, T>
+                            : route_kernel<32, T>;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_kernel(kern, dim3((unsigned)blocks), dim3(warps * 32), smem, c.stream, pdl_enabled(), p, tokens, fuse);
+}
+cudaError_t run_route_of(const LaunchCtx& c, const RouteParams& p, int blocks, int tokens, bool fuse) {
+    return p.dtype == 0 ? run_route<float>(c, p, blocks, tokens, fuse) : p.dtype == 1 ? run_route<__nv_bfloat16>(c, p, blocks, tokens, fuse) : run_route<__half>(c, p, blocks, tokens, fuse);
+}
+
+int run_place(const char* kn, const LaunchCtx& c, const int* ids, float* w, int* bucket_rows, int* base, int* offsets, const int* hist, int pairs, int n_exp,
+              int topk, int blocks, int per_block) {
+    const size_t smem = (size_t)n_exp * 4 * (2 + 32);
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return cuda_fail(kn, e);
+    }
+    const cudaError_t e = launch_kernel(plan_place_kernel, dim3(blocks), dim3(1024), smem, c.stream, pdl_enabled(), ids, w, bucket_rows, base, offsets, hist,
+                                        pairs, n_exp, topk, per_block);
+    return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
+}
+
+// arguments of the choice; `a` begins with rows
+int read_route(const char* kn, RouteParams& p, const uint64_t* a) {
+    p.rows = arg_i32(a[0]);
+    p.n_exp = arg_i32(a[1]);
+    p.topk = arg_i32(a[2]);
+    p.n_group = arg_i32(a[3]);
+    p.topk_group = arg_i32(a[4]);
+    p.group_top = arg_i32(a[5]);
+    const int score = arg_i32(a[6]), renorm = arg_i32(a[7]);
+    p.scale = arg_f32(a[8]);
+    p.dtype = arg_i32(a[9]);
     FM_REQUIRE(p.rows >= 0 && p.n_exp >= 1 && p.n_exp <= kMaxExperts, kn, "rows=%d n_exp=%d: 1..%d experts", p.rows, p.n_exp, kMaxExperts);
     FM_REQUIRE(p.n_group >= 1 && p.n_group <= kMaxGroups && p.n_exp % p.n_group == 0, kn, "n_group=%d must divide n_exp=%d and be at most %d",
                p.n_group, p.n_exp, kMaxGroups);
@@ -318,129 +682,88 @@ int launch_route(const LaunchCtx& c, const uint64_t* a) {
                "topk=%d: at most %d, and at most the experts of the kept groups", p.topk, kMaxTopk);
     FM_REQUIRE(p.group_top == 1 || p.group_top == 2, kn, "group_top=%d: 1 or 2", p.group_top);
     FM_REQUIRE((score == 0 || score == 1) && (renorm == 0 || renorm == 1), kn, "score=%d renorm=%d: 0 or 1", score, renorm);
-    FM_REQUIRE(dtype >= 0 && dtype <= 2, kn, "dtype=%d: 0 f32, 1 bf16, 2 f16", dtype);
+    FM_REQUIRE(p.dtype >= 0 && p.dtype <= 2, kn, "dtype=%d: 0 f32, 1 bf16, 2 f16", p.dtype);
     p.sigmoid = score == 1;
     p.renorm = renorm == 1;
     p.group_size = p.n_exp / p.n_group;
+    int vpl = 1;
+    while (vpl * 32 < p.n_exp) vpl *= 2;
+    const int lanes = p.group_size / vpl;
+    p.group_lanes = p.group_size % vpl == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+    const size_t es = p.dtype == 0 ? 4 : 2, pairs = (size_t)p.rows * p.topk;
+    FM_REQUIRE(pairs <= (1u << 30), kn, "rows * topk = %zu: at most 2^30 pairs", pairs);
     if (p.rows == 0) return FM_OK;
-    const size_t es = dtype == 0 ? 4 : 2, pairs = (size_t)p.rows * p.topk;
-    FM_REQUIRE(pairs <= 0x7fffffff, kn, "rows * topk exceeds 2^31 - 1");
     FM_REQUIRE(aligned(p.logits, es) && aligned(p.bias, 4) && aligned(p.ids, 4) && aligned(p.weights, 4), kn, "misaligned pointer");
     FM_RANGE(p.logits, (size_t)p.rows * p.n_exp * es, kn, "logits");
     if (p.bias) FM_RANGE(p.bias, (size_t)p.n_exp * 4, kn, "bias");
     FM_RANGE(p.ids, pairs * 4, kn, "ids");
     FM_RANGE(p.weights, pairs * 4, kn, "weights");
-    const cudaError_t e = dtype == 0 ? run_route<float>(c, p) : dtype == 1 ? run_route<__nv_bfloat16>(c, p) : run_route<__half>(c, p);
+    p.vector = aligned(p.logits, 16) && (size_t)p.n_exp * es % 16 == 0;
+    return FM_OK;
+}
+
+// blocks of a routing launch: one to an SM, a token to a block at least
+void route_shape(const LaunchCtx& c, int rows, int& blocks, int& tokens) {
+    tokens = (rows + c.sm_count - 1) / c.sm_count;
+    blocks = (rows + tokens - 1) / tokens;
+}
+
+int launch_route(const LaunchCtx& c, const uint64_t* a) {
+    const char* kn = "moe_route_k";
+    RouteParams p = {};
+    p.logits = arg_ptr<const void>(a[0]);
+    p.bias = arg_ptr<const float>(a[1]);
+    p.ids = arg_ptr<int>(a[2]);
+    p.weights = arg_ptr<float>(a[3]);
+    const int rc = read_route(kn, p, a + 4);
+    if (rc != FM_OK || p.rows == 0) return rc;
+    int blocks, tokens;
+    route_shape(c, p.rows, blocks, tokens);
+    const cudaError_t e = run_route_of(c, p, blocks, tokens, false);
     return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
 }
 
-// ------------------------------------------------------------------------------------------------------ the plan
-// A block takes kChunk consecutive pairs, a warp kChunk / 8 of them in batches of 32.  The slot of a pair is
-//   (pairs of smaller experts) + (pairs of its expert in earlier blocks, warps, batches and lanes),
-// so the order is that of the pair indices whatever the scheduling: no atomics decide a position.
-constexpr int kPlanThreads = 256, kPlanWarps = kPlanThreads / 32, kChunk = 2048, kPerWarp = kChunk / kPlanWarps;
-
-__device__ __forceinline__ int pair_expert(const int* ids, const float* w, int i, int pairs, int n_exp) {
-    if (i >= pairs) return -1;
-    const int e = ids[i];
-    return e >= 0 && e < n_exp && w[i] != 0.f ? e : -1;
+// ranges of a plan's arrays
+int check_plan(const char* kn, const int* bucket_rows, const int* base, const int* offsets, size_t pairs, int n_exp) {
+    FM_REQUIRE(aligned(bucket_rows, 4) && aligned(base, 4) && aligned(offsets, 4), kn, "misaligned pointer");
+    FM_RANGE(bucket_rows, pairs * 4, kn, "bucket_rows");
+    FM_RANGE(base, pairs * 4, kn, "base");
+    FM_RANGE(offsets, (size_t)(n_exp + 1) * 4, kn, "offsets");
+    return FM_OK;
 }
 
-// hist[block][n_exp]
-__global__ void __launch_bounds__(kPlanThreads)
-plan_count_kernel(const int* __restrict__ ids, const float* __restrict__ w, int* __restrict__ hist, int pairs, int n_exp) {
-    extern __shared__ int count[];
-    pdl_wait();
-    for (int e = threadIdx.x; e < n_exp; e += kPlanThreads) count[e] = 0;
-    __syncthreads();
-    const int lo = blockIdx.x * kChunk;
-    for (int i = lo + threadIdx.x; i < lo + kChunk; i += kPlanThreads) {
-        const int e = pair_expert(ids, w, i, pairs, n_exp);
-        if (e >= 0) atomicAdd(&count[e], 1);                          // (integers: the order does not matter)
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < n_exp; e += kPlanThreads) hist[(size_t)blockIdx.x * n_exp + e] = count[e];
-    pdl_launch_dependents();
+int no_rows(const char* kn, const LaunchCtx& c, int* offsets, int n_exp) {
+    const cudaError_t e = cudaMemsetAsync(offsets, 0, (size_t)(n_exp + 1) * 4, c.stream);
+    return e == cudaSuccess ? FM_OK : cuda_fail(kn, e);
 }
 
-__global__ void __launch_bounds__(kPlanThreads)
-plan_place_kernel(const int* __restrict__ ids, float* __restrict__ w, int* __restrict__ bucket_rows, int* __restrict__ base,
-                  int* __restrict__ offsets, const int* __restrict__ hist, int pairs, int n_exp, int topk) {
-    extern __shared__ int sm[];
-    int* start = sm;                                                  // [n_exp] first slot of this block's pairs
-    int* cnt = sm + n_exp;                                            // [kPlanWarps][n_exp]
-    __shared__ int warp_total[kPlanWarps];
-    pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int i = threadIdx.x; i < kPlanWarps * n_exp; i += kPlanThreads) cnt[i] = 0;
-    // totals per expert over all blocks and over the earlier ones; exclusive scan over the experts
-    int carry = 0;
-    for (int e0 = 0; e0 < n_exp; e0 += kPlanThreads) {
-        const int e = e0 + threadIdx.x;
-        int total = 0, before = 0;
-        if (e < n_exp)
-            for (int b = 0; b < (int)gridDim.x; b++) {
-                const int h = hist[(size_t)b * n_exp + e];
-                if (b < (int)blockIdx.x) before += h;
-                total += h;
-            }
-        int inc = total;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += t;
-        }
-        __syncthreads();
-        if (lane == 31) warp_total[warp] = inc;
-        __syncthreads();
-        int lower = carry, all = 0;
-        for (int k = 0; k < kPlanWarps; k++) {
-            if (k < warp) lower += warp_total[k];
-            all += warp_total[k];
-        }
-        if (e < n_exp) {
-            start[e] = lower + inc - total + before;
-            if (blockIdx.x == 0) {
-                offsets[e] = lower + inc - total;
-                if (e == n_exp - 1) offsets[n_exp] = lower + inc;
-            }
-        }
-        carry += all;
+int launch_route_plan(const LaunchCtx& c, const uint64_t* a) {
+    const char* kn = "moe_route_plan_k";
+    RouteParams p = {};
+    p.logits = arg_ptr<const void>(a[0]);
+    p.bias = arg_ptr<const float>(a[1]);
+    p.ids = arg_ptr<int>(a[2]);
+    p.weights = arg_ptr<float>(a[3]);
+    p.bucket_rows = arg_ptr<int>(a[4]);
+    p.base = arg_ptr<int>(a[5]);
+    p.offsets = arg_ptr<int>(a[6]);
+    int rc = read_route(kn, p, a + 7);
+    if (rc != FM_OK) return rc;
+    const size_t pairs = (size_t)p.rows * p.topk;
+    if ((rc = check_plan(kn, p.bucket_rows, p.base, p.offsets, pairs, p.n_exp)) != FM_OK) return rc;
+    if (p.rows == 0) return no_rows(kn, c, p.offsets, p.n_exp);
+    int blocks, tokens;
+    route_shape(c, p.rows, blocks, tokens);
+    const bool fuse = pairs <= kFusePairs && p.n_exp <= kFuseExperts;
+    if (!fuse) {
+        p.hist = static_cast<int*>(engine_scratch((size_t)blocks * p.n_exp * 4));
+        FM_REQUIRE(p.hist, kn, "the engine workspace cannot grow to %zu bytes here (inside a capture: raise FM_SCRATCH_MB)", (size_t)blocks * p.n_exp * 4);
     }
-    __syncthreads();
-    // this warp's pairs per expert
-    const int lo = blockIdx.x * kChunk + warp * kPerWarp;
-    for (int i = lo + lane; i < lo + kPerWarp; i += 32) {
-        const int e = pair_expert(ids, w, i, pairs, n_exp);
-        if (e >= 0) atomicAdd(&cnt[warp * n_exp + e], 1);
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < n_exp; e += kPlanThreads) {
-        int at = start[e];
-        for (int k = 0; k < kPlanWarps; k++) {
-            const int h = cnt[k * n_exp + e];
-            cnt[k * n_exp + e] = at;
-            at += h;
-        }
-    }
-    __syncthreads();
-    for (int i0 = lo; i0 < lo + kPerWarp && i0 < pairs; i0 += 32) {
-        const int i = i0 + lane;
-        const int e = pair_expert(ids, w, i, pairs, n_exp);
-        const uint32_t peers = __match_any_sync(0xffffffffu, e);
-        const int rank = __popc(peers & ((1u << lane) - 1u));
-        int slot = 0;
-        if (e >= 0) slot = cnt[warp * n_exp + e] + rank;
-        __syncwarp();
-        if (e >= 0 && rank == 0) cnt[warp * n_exp + e] += __popc(peers);
-        __syncwarp();
-        if (i < pairs) {
-            base[i] = slot;
-            if (e >= 0) bucket_rows[slot] = i / topk;
-            else w[i] = 0.f;
-        }
-    }
-    pdl_launch_dependents();
+    const cudaError_t e = run_route_of(c, p, blocks, tokens, fuse);
+    if (e != cudaSuccess) return cuda_fail(kn, e);
+    rc = after_launch(kn);
+    if (rc != FM_OK || fuse) return rc;
+    return run_place(kn, c, p.ids, p.weights, p.bucket_rows, p.base, p.offsets, p.hist, (int)pairs, p.n_exp, p.topk, blocks, tokens * p.topk);
 }
 
 int launch_plan(const LaunchCtx& c, const uint64_t* a) {
@@ -454,29 +777,31 @@ int launch_plan(const LaunchCtx& c, const uint64_t* a) {
     FM_REQUIRE(rows >= 0 && n_exp >= 1 && n_exp <= kMaxExperts && topk >= 1 && topk <= kMaxTopk, kn,
                "rows=%d n_exp=%d topk=%d: 1..%d experts, 1..%d choices", rows, n_exp, topk, kMaxExperts, kMaxTopk);
     const size_t pairs = (size_t)rows * topk;
-    FM_REQUIRE(pairs <= 0x7fffffff - kChunk, kn, "rows * topk exceeds what 32-bit slots can name");
-    FM_REQUIRE(aligned(ids, 4) && aligned(w, 4) && aligned(bucket_rows, 4) && aligned(base, 4) && aligned(offsets, 4), kn, "misaligned pointer");
+    FM_REQUIRE(pairs <= (1u << 30), kn, "rows * topk = %zu: at most 2^30 pairs", pairs);
+    FM_REQUIRE(aligned(ids, 4) && aligned(w, 4), kn, "misaligned pointer");
     FM_RANGE(ids, pairs * 4, kn, "ids");
     FM_RANGE(w, pairs * 4, kn, "weights");
-    FM_RANGE(bucket_rows, pairs * 4, kn, "bucket_rows");
-    FM_RANGE(base, pairs * 4, kn, "base");
-    FM_RANGE(offsets, (size_t)(n_exp + 1) * 4, kn, "offsets");
-    const int blocks = pairs ? (int)((pairs + kChunk - 1) / kChunk) : 1;   // (no rows: the offsets are still written)
+    const int rc = check_plan(kn, bucket_rows, base, offsets, pairs, n_exp);
+    if (rc != FM_OK) return rc;
+    if (rows == 0) return no_rows(kn, c, offsets, n_exp);
+    const int most = c.sm_count;
+    int per_block = (int)((pairs + most - 1) / most);
+    if (per_block < 512) per_block = 512;
+    const int blocks = (int)((pairs + per_block - 1) / per_block);
     int* hist = static_cast<int*>(engine_scratch((size_t)blocks * n_exp * 4));
     FM_REQUIRE(hist, kn, "the engine workspace cannot grow to %zu bytes here (inside a capture: raise FM_SCRATCH_MB)", (size_t)blocks * n_exp * 4);
-    cudaError_t e = launch_kernel(plan_count_kernel, dim3(blocks), dim3(kPlanThreads), (size_t)n_exp * 4, c.stream, pdl_enabled(), ids, w,
-                                  hist, (int)pairs, n_exp);
+    const cudaError_t e = launch_kernel(plan_count_kernel, dim3(blocks), dim3(kThreads), (size_t)n_exp * 4, c.stream, pdl_enabled(), ids, w, hist, (int)pairs,
+                                        n_exp, per_block);
     if (e != cudaSuccess) return cuda_fail(kn, e);
-    const int rc = after_launch(kn);
-    if (rc != FM_OK) return rc;
-    e = launch_kernel(plan_place_kernel, dim3(blocks), dim3(kPlanThreads), (size_t)n_exp * 4 * (1 + kPlanWarps), c.stream, pdl_enabled(), ids, w,
-                      bucket_rows, base, offsets, hist, (int)pairs, n_exp, topk);
-    return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
+    const int rc2 = after_launch(kn);
+    if (rc2 != FM_OK) return rc2;
+    return run_place(kn, c, ids, w, bucket_rows, base, offsets, hist, (int)pairs, n_exp, topk, blocks, per_block);
 }
 
 const KernelEntry kRoute[] = {
     {"moe_route_k", 14, launch_route, "ppppiiiiiiiifi"},
     {"moe_plan_k", 8, launch_plan, "pppppiii"},
+    {"moe_route_plan_k", 17, launch_route_plan, "pppppppiiiiiiiifi"},
 };
 
 }  // namespace

@@ -168,10 +168,8 @@ class MoERouter:
         pairs4 = max(1, rows * self.topk) * 4
         b = {n: self.ws.buffer(f"{self.tag}.{n}", pairs4) for n in ("ids", "weights", "bucket_rows", "base")}
         plan = MoEPlan(rows, self.topk, self.n_exp, offsets=self.ws.buffer(self.tag + ".offsets", (self.n_exp + 1) * 4), **b)
-        self.rt.launch("moe_route_k", 1, 1, [int(logits_dev), self.bias, plan.ids, plan.weights, rows, self.n_exp, self.topk,
-                                             *self._tail])
-        self.rt.launch("moe_plan_k", 1, 1, [plan.ids, plan.weights, plan.bucket_rows, plan.base, plan.offsets, rows,
-                                            self.n_exp, self.topk])
+        self.rt.launch("moe_route_plan_k", 1, 1, [int(logits_dev), self.bias, plan.ids, plan.weights, plan.bucket_rows, plan.base,
+                                                  plan.offsets, rows, self.n_exp, self.topk, *self._tail])
         if sync:
             self.rt.sync()
         return plan

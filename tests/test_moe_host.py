@@ -80,7 +80,7 @@ def test_launch_sequence_and_argument_counts():
     block = MoEMLP(rt, router, ExpertLinear(rt, 4, 128, 256, 1, 2, act="silu", gated=True), ExpertLinear(rt, 4, 256, 128, 1, 2))
     block.forward_device(64, 128, 5)
     names = [l[0] for l in rt.launches]
-    assert names == ["moe_route_k", "moe_plan_k", "memset", "quant_act", "moe_linear_w4a8_k", "quant_act", "moe_linear_w4a8_k",
+    assert names == ["moe_route_plan_k", "memset", "quant_act", "moe_linear_w4a8_k", "quant_act", "moe_linear_w4a8_k",
                      "moe_combine_gather_k"]
     FusedLinear(rt, 4, 128, 64, 128, bias=77).forward_device(64, 3, residual_dev=4096)
     for name, _grid, _wg, nargs in rt.launches:
