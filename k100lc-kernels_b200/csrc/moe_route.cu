@@ -77,11 +77,15 @@ __device__ __forceinline__ float rcp_approx(float x) {
     return d;
 }
 
-// Two fp32 keys of at most this magnitude are told apart for certain when they are this far from each other: the score is
-// at most 1, its exp within 2^-22 and, the argument x log2(e) being rounded, within |x| 2^-24, of which the score sees at
-// most x exp(-x) <= 0.37; the reciprocal is within 2^-23, a sum of up to 1024 scores (32 in turn, then five halvings) within
-// 37 * 2^-24; adding the bias rounds by at most 2^-24 of the key.  2^-17 is over twice the sum of these.
-__device__ __forceinline__ float resolution(float most) { return 7.6293945e-6f + 2.3841858e-7f * most; }
+// Two fp32 keys of at most this magnitude are told apart for certain when they are this far from each other.
+// sigmoid: exp is within 2^-22 and, its argument x log2(e) being rounded, within |x| 2^-24, of which s (1 - s) <= 1/4 reaches
+// the score; 1 + exp rounds by 2^-24, the reciprocal by 2^-23: 3e-7 together, twice that for two scores.  softmax: a sum of up
+// to 1024 exps (32 in turn, then five halvings) is within 37 * 2^-24 of its value besides: 2.8e-6, twice that.  Adding the
+// bias rounds by 2^-24 of the key, the position in its lowest bits takes up to VPL steps of 2^-23.
+template <int VPL>
+__device__ __forceinline__ float resolution(const RouteParams& p, float most) {
+    return (!p.bias && p.group_top == 1 ? 0.f : p.sigmoid ? 1e-6f : 6e-6f) + (VPL + 2) * 1.1920929e-7f * most;
+}
 
 // ---- the decision in fp64: lane's experts lane * VPL + i, plain loops; taken for the few tokens that fp32 cannot decide
 template <int VPL>
@@ -176,13 +180,20 @@ __device__ __noinline__ int decide64(const RouteParams& p, const float* __restri
 // exp and 1 / x to 2^-21 at least: good enough to order by (see `resolution`), not for the weights
 __device__ __forceinline__ float fast_exp(float x) { return exp2f_approx(x * 1.4426950f); }
 
-// Sorts the lane's keys, descending, equal keys by ascending position; `at` holds the positions, four bits each.
+// A key carries its position in the lane in its lowest bits, the first highest, so that a lane's keys are distinct, equal
+// values keep the order of their indices, and a sort moves one word.  The bits cost the key at most 2^-18 of its value;
+// `resolution` allows for it.  (16-bit logits have no bits there.)
 template <int VPL>
-__device__ __forceinline__ void sort_lane(uint32_t (&k)[VPL], uint32_t& order) {
-    uint32_t at[VPL];
-#pragma unroll
-    for (int i = 0; i < VPL; i++) at[i] = i;
-    // Batcher's odd-even merge sort (1968)
+__device__ __forceinline__ uint32_t key_of(float v, int i) {
+    const uint32_t o = ordered(v);
+    return o ? (o & ~(uint32_t)(VPL - 1)) | (uint32_t)(VPL - 1 - i) : 0u;
+}
+template <int VPL>
+__device__ __forceinline__ float value_of(uint32_t key) { return key_value(key & ~(uint32_t)(VPL - 1)); }
+
+// Sorts the lane's keys, descending: Batcher's odd-even merge sort (1968).
+template <int VPL>
+__device__ __forceinline__ void sort_lane(uint32_t (&k)[VPL]) {
 #pragma unroll
     for (int p = 1; p < VPL; p <<= 1)
 #pragma unroll
@@ -192,63 +203,39 @@ __device__ __forceinline__ void sort_lane(uint32_t (&k)[VPL], uint32_t& order) {
 #pragma unroll
                 for (int i = 0; i < q; i++)
                     if (i + j + q < VPL && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
-                        const int a = i + j, b = i + j + q;
-                        const bool swap = k[b] > k[a] || (k[b] == k[a] && at[b] < at[a]);
-                        const uint32_t ka = k[a], ia = at[a];
-                        k[a] = swap ? k[b] : ka;
-                        at[a] = swap ? at[b] : ia;
-                        k[b] = swap ? ka : k[b];
-                        at[b] = swap ? ia : at[b];
+                        const uint32_t hi = max(k[i + j], k[i + j + q]), lo = min(k[i + j], k[i + j + q]);
+                        k[i + j] = hi;
+                        k[i + j + q] = lo;
                     }
-    order = 0;
-#pragma unroll
-    for (int i = 0; i < VPL; i++) order |= at[i] << (4 * (i & 7));
 }
 
-// The topk largest keys of the warp in order, as positions lane * VPL + i, and (with `more`) the key after them: lane j gets
-// the j-th position (-1: none) and key.  Keys of up to eight a lane come sorted (`order`: their positions).
+// The largest keys of the warp in order, from the lanes' sorted lists: lane j gets the j-th position (-1: none) and key.
 template <int VPL>
-__device__ __forceinline__ int pick(int rounds, uint32_t (&key)[VPL], uint32_t order, uint32_t& kept) {
+__device__ __forceinline__ int pick(int rounds, uint32_t (&key)[VPL], uint32_t& kept) {
     const int lane = threadIdx.x & 31;
-    int mine = -1;
+    int whose = -1;
     kept = 0;
     for (int j = 0; j < rounds; j++) {
-        uint32_t best = key[0];
-        if (VPL > 8) {
-#pragma unroll
-            for (int i = 1; i < VPL; i++) best = max(best, key[i]);
-        }
+        const uint32_t best = key[0] & ~(uint32_t)(VPL - 1);
         const uint32_t top = __reduce_max_sync(0xffffffffu, best);
         if (top == 0) break;
         const int from = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
-        int at = (int)(order & 15u);
-        const bool hit = lane == from;
-        if (VPL <= 8) {                                               // sorted: the next one moves up
+        const uint32_t k = __shfl_sync(0xffffffffu, key[0], from);
+        const bool hit = lane == from;                                // its next one moves up
 #pragma unroll
-            for (int i = 0; i + 1 < VPL; i++) key[i] = hit ? key[i + 1] : key[i];
-            key[VPL - 1] = hit ? 0u : key[VPL - 1];
-            order = hit ? order >> 4 : order;
-        } else {
-            at = 0;
-#pragma unroll
-            for (int i = VPL - 1; i >= 0; i--)
-                if (key[i] == top) at = i;
-#pragma unroll
-            for (int i = 0; i < VPL; i++)
-                if (hit && i == at) key[i] = 0;
-        }
-        const int e = from * VPL + __shfl_sync(0xffffffffu, at, from);
+        for (int i = 0; i + 1 < VPL; i++) key[i] = hit ? key[i + 1] : key[i];
+        key[VPL - 1] = hit ? 0u : key[VPL - 1];
         if (lane == j) {
-            mine = e;
-            kept = top;
+            whose = from;
+            kept = k;
         }
     }
-    return mine;
+    return whose < 0 ? -1 : whose * VPL + (VPL - 1 - (int)(kept & (uint32_t)(VPL - 1)));
 }
 
-// Which groups stay, as a mask.  a, b: the two best of the lane's group (group_lanes > 0) or of group `lane`.  gap: the distance
-// between the worst group kept and the best one dropped.
-__device__ __forceinline__ uint32_t best_groups(const RouteParams& p, float a, float b, float& gap) {
+// Which groups stay, as a mask of the lanes that speak for them (the first of a group).  a, b: the two best of the lane's group (group_lanes > 0) or of group `lane`.  gap: the distance
+// between the worst group kept and the best one dropped; most: the largest magnitude of the numbers that make the groups' worths.
+__device__ __forceinline__ uint32_t best_groups(const RouteParams& p, float a, float b, float& gap, float& most) {
     const int lane = threadIdx.x & 31, lanes = p.group_lanes;
     for (int o = 1; o < lanes; o <<= 1) {
         const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
@@ -258,21 +245,32 @@ __device__ __forceinline__ uint32_t best_groups(const RouteParams& p, float a, f
     const int group = lanes > 0 ? lane / lanes : lane;
     const bool speaks = group < p.n_group && (lanes <= 1 || lane % lanes == 0);          // one lane of a group speaks for it
     uint32_t w = speaks ? ordered(p.group_top == 2 && b > -INFINITY ? a + b : a) : 0u;
-    uint32_t kept = 0;
-    float last = INFINITY, next = -INFINITY;
-    for (int k = 0; k <= p.topk_group; k++) {
-        const uint32_t best = __reduce_max_sync(0xffffffffu, w);
-        if (k == p.topk_group) {
-            next = key_value(best);
-            break;
+    uint32_t kept = 0, last = 0, next = 0;
+    if (p.n_group <= 4 * p.topk_group) {                              // a group's rank is the number of better ones
+        int rank = 0;
+        for (int g = 0; g < p.n_group; g++) {
+            const uint32_t t = __shfl_sync(0xffffffffu, w, lanes > 0 ? g * lanes : g);
+            rank += t > w || (t == w && g < group);
         }
-        if (best == 0) break;                                         // the other groups are empty
-        const int from = __ffs(__ballot_sync(0xffffffffu, w == best)) - 1;
-        kept |= 1u << (lanes > 0 ? from / lanes : from);
-        last = key_value(best);
-        if (lane == from) w = 0;
+        kept = __ballot_sync(0xffffffffu, speaks && rank < p.topk_group && w != 0);
+        last = __reduce_max_sync(0xffffffffu, speaks && rank == p.topk_group - 1 ? w : 0u);
+        next = __reduce_max_sync(0xffffffffu, speaks && rank == p.topk_group ? w : 0u);
+    } else {
+        uint32_t left = w;
+        for (int k = 0; k < p.topk_group; k++) {
+            last = __reduce_max_sync(0xffffffffu, left);
+            if (last == 0) break;                                     // the other groups are empty
+            const uint32_t who = __ballot_sync(0xffffffffu, left == last);
+            kept |= who & (0u - who);                                 // the first
+            if ((who & (0u - who)) >> lane & 1u) left = 0;
+        }
+        next = __reduce_max_sync(0xffffffffu, left);
     }
-    gap = last - next;
+    const float l = last ? key_value(last) : INFINITY, n = key_value(next);
+    gap = l - n;
+    // (of a group's two numbers one may be large and negative: their magnitudes bound the error of the sum)
+    const float size = speaks ? fmaxf(fabsf(a), b > -INFINITY ? fabsf(b) : 0.f) : 0.f;
+    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size < INFINITY ? size : 0.f)));
     return kept;
 }
 
@@ -300,9 +298,9 @@ __device__ __forceinline__ void load_logits(const RouteParams& p, size_t row, fl
 
 // One token: lane j < topk gets its j-th expert and weight.  Keys are formed and ordered in fp32; a token where two that
 // matter lie within the error of fp32 is decided again in fp64, so that the choice is that of the exact keys at fp32's cost.
-// bias: the lane's, `most`: the largest magnitude that a finite key can have.
+// bias: the lane's.
 template <int VPL, typename T>
-__device__ __forceinline__ void route_token(const RouteParams& p, size_t row, const float (&bias)[VPL], float most, double* stage, int& id, float& weight) {
+__device__ __forceinline__ void route_token(const RouteParams& p, size_t row, const float (&bias)[VPL], double* stage, int& id, float& weight) {
     const int lane = threadIdx.x & 31;
     float x[VPL], s[VPL];                                             // logits; scores to order by
     load_logits<VPL, T>(p, row, x);
@@ -329,9 +327,10 @@ __device__ __forceinline__ void route_token(const RouteParams& p, size_t row, co
 #pragma unroll
         for (int i = 0; i < VPL; i++) s[i] = rcp_approx(1.f + fast_exp(-x[i]));
     }
-    uint32_t key[VPL], order = 0, kept = 0;
+    uint32_t key[VPL], kept;
 #pragma unroll
-    for (int i = 0; i < VPL; i++) key[i] = ordered(!p.bias ? x[i] : x[i] > -INFINITY ? s[i] + bias[i] : -INFINITY);
+    for (int i = 0; i < VPL; i++) key[i] = key_of<VPL>(!p.bias ? x[i] : x[i] > -INFINITY ? s[i] + bias[i] : -INFINITY, i);
+    const bool check = p.bias || sizeof(T) == 4;                      // (16-bit logits themselves are exact keys)
     bool near = false;
     float a = -INFINITY, b = -INFINITY;                               // the two best of the lane
     if (by_score) {
@@ -346,7 +345,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, size_t row, co
         float* list = reinterpret_cast<float*>(stage);
 #pragma unroll
         for (int i = 0; i < VPL; i++)
-            if (lane * VPL + i < p.n_exp) list[lane * VPL + i] = by_score && key[i] ? s[i] : key_value(key[i]);
+            if (lane * VPL + i < p.n_exp) list[lane * VPL + i] = by_score && key[i] ? s[i] : value_of<VPL>(key[i]);
         __syncwarp();
         a = b = -INFINITY;
         if (lane < p.n_group)
@@ -356,48 +355,39 @@ __device__ __forceinline__ void route_token(const RouteParams& p, size_t row, co
                 a = fmaxf(a, t);
             }
         __syncwarp();
-        float gap;
-        const uint32_t groups = best_groups(p, a, b, gap);
-        near = need && !(gap > 2.f * resolution(most));               // (a group's worth is a sum of two)
+        float gap, most;
+        const uint32_t groups = best_groups(p, a, b, gap, most);
+        near = (check || by_score) && !(gap > 2.f * resolution<VPL>(p, most));       // (a group's worth is a sum of two)
 #pragma unroll
         for (int i = 0; i < VPL; i++) {
             const int e = lane * VPL + i;
-            if (e < p.n_exp && !((groups >> (e / p.group_size)) & 1u)) key[i] = 0;
+            if (e < p.n_exp && !((groups >> (e / p.group_size)) & 1u)) key[i] = 0;       // (lane g speaks for group g)
         }
     }
-    if (VPL <= 8) sort_lane<VPL>(key, order);
+    sort_lane<VPL>(key);
     if (p.n_group > 1 && p.group_lanes > 0) {
         if (!by_score) {
-            if (VPL <= 8) {
-                a = key_value(key[0]);
-                if (VPL > 1) b = key_value(key[VPL > 1 ? 1 : 0]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < VPL; i++) {
-                    const float t = key_value(key[i]);
-                    b = fmaxf(b, fminf(a, t));
-                    a = fmaxf(a, t);
-                }
-            }
+            a = value_of<VPL>(key[0]);
+            if (VPL > 1) b = value_of<VPL>(key[VPL > 1 ? 1 : 0]);
         }
-        float gap;
-        const uint32_t groups = best_groups(p, a, b, gap);
-        near = need && !(gap > 2.f * resolution(most));
-        if (!((groups >> ((lane / p.group_lanes) & 31)) & 1u)) {
+        float gap, most;
+        const uint32_t groups = best_groups(p, a, b, gap, most);
+        near = (check || by_score) && !(gap > 2.f * resolution<VPL>(p, most));
+        if (!((groups >> (lane & ~(p.group_lanes - 1))) & 1u)) {
 #pragma unroll
             for (int i = 0; i < VPL; i++) key[i] = 0;
         }
     }
-    id = pick<VPL>(min(p.topk + (p.bias ? 1 : 0), 32), key, order, kept);
-    if (p.bias) {
-        // (with 32 choices the key after them has no lane: two of all are then compared below 32 only, and fp64 decides)
-        const float v = key_value(kept), prev = __shfl_up_sync(0xffffffffu, v, 1);
+    id = pick<VPL>(min(p.topk + (check ? 1 : 0), 32), key, kept);
+    if (check) {
+        const float v = value_of<VPL>(kept), prev = __shfl_up_sync(0xffffffffu, v, 1);
         const int before = __shfl_up_sync(0xffffffffu, id, 1);
-        bool close = lane > 0 && lane <= p.topk && id >= 0 && !(prev - v > resolution(fmaxf(fabsf(v), fabsf(prev))));
+        bool close = lane > 0 && lane <= p.topk && id >= 0 && !(prev - v > resolution<VPL>(p, fmaxf(fabsf(v), fabsf(prev))));
         if (close) {                                                  // equal inputs are equal keys: the order of the index is right
             const T* in = reinterpret_cast<const T*>(p.logits) + row * p.n_exp;
-            close = !(logit_at(in, id) == logit_at(in, before) && p.bias[id] == p.bias[before]);
+            close = !(logit_at(in, id) == logit_at(in, before) && (!p.bias || p.bias[id] == p.bias[before]));
         }
+        // (the key after 32 choices has no lane to compare it in)
         near = near || p.topk == 32 || __any_sync(0xffffffffu, close);
     }
     if (near) {
@@ -500,7 +490,7 @@ __device__ unsigned g_blocks_done;                   // blocks of a fused launch
 // Block b routes the tokens [b * tokens, (b + 1) * tokens), a warp a token at a time.  With a plan: few pairs are placed by
 // the block that finishes last (fuse), otherwise every block counts its pairs of each expert for plan_place_kernel.
 template <int VPL, typename T>
-__global__ void __launch_bounds__(1024, 1)
+__global__ void __launch_bounds__(VPL <= 8 ? 1024 : 512, 1)
 route_kernel(const RouteParams p, int tokens, bool fuse) {
     extern __shared__ double dyn[];                                   // [warps][n_exp] where there are groups; then ints
     __shared__ int next, part[32];
@@ -512,21 +502,16 @@ route_kernel(const RouteParams p, int tokens, bool fuse) {
     if (p.hist)
         for (int e = threadIdx.x; e < p.n_exp; e += blockDim.x) count[e] = 0;
     if (threadIdx.x == 0) next = warps;
-    float bias[VPL], most = 1.f;
+    float bias[VPL];
 #pragma unroll
-    for (int i = 0; i < VPL; i++) {
-        const int e = lane * VPL + i;
-        bias[i] = p.bias && e < p.n_exp ? p.bias[e] : 0.f;
-        if (fabsf(bias[i]) < INFINITY) most = fmaxf(most, 1.f + fabsf(bias[i]));
-    }
-    if (p.bias) most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+    for (int i = 0; i < VPL; i++) bias[i] = p.bias && lane * VPL + i < p.n_exp ? p.bias[lane * VPL + i] : 0.f;
     __syncthreads();
     const int row0 = blockIdx.x * tokens, rows = min(tokens, p.rows - row0);
     for (int t = warp; t < rows;) {                                   // (whichever warp is free takes the next token)
         const size_t row = (size_t)row0 + t;
         int id;
         float w;
-        route_token<VPL, T>(p, row, bias, most, stage, id, w);
+        route_token<VPL, T>(p, row, bias, stage, id, w);
         if (lane < p.topk) {
             p.ids[row * p.topk + lane] = id;
             p.weights[row * p.topk + lane] = w;
@@ -631,10 +616,10 @@ constexpr int kFuseExperts = 256;
 
 template <typename T>
 cudaError_t run_route(const LaunchCtx& c, const RouteParams& p, int blocks, int tokens, bool fuse) {
-    int warps = tokens < 32 ? tokens : 32;
+    const int vpl = (p.n_exp + 31) / 32, most = vpl <= 8 ? 32 : 16;
+    int warps = tokens < most ? tokens : most;
     if (fuse && warps < 8) warps = 8;                                 // (they place the pairs)
     const size_t smem = (p.n_group > 1 ? (size_t)warps * p.n_exp * 8 : 0) + (p.hist ? (size_t)p.n_exp * 4 : 0) + (fuse ? (size_t)p.n_exp * 4 * (1 + warps) : 0);
-    const int vpl = (p.n_exp + 31) / 32;
     auto kern = vpl <= 1   ? route_kernel<1, T>
                 : vpl <= 2 ? route_kernel<2, T>
                 : vpl <= 4 ? route_kernel<4, T>
