@@ -8,14 +8,13 @@
 // returns float(I) and the epilogue needs no conversion (with kind::i8 the conversions, 16 a clock per SM, take four
 // times as long as the MMAs).
 //
-// Roles of the 24 warps of the persistent CTA, joined by mbarriers (every wait is bounded):
+// Roles of the 20 warps of the persistent CTA, joined by mbarriers (every wait is bounded):
 //   * one warp copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring;
 //   * eight warps expand them: a thread owns a weight row, reads its 64 bytes, turns nibbles into f16 pairs with four
 //     logic and four arithmetic instructions a word, and writes them to tensor memory, from where the MMA takes its A
 //     operand: no shared-memory traffic for the wide operand, which would otherwise bound the tile (128 bytes a clock);
 //   * one warp copies the rows of x by TMA: f16, put into bucket order and into the k order of the nibble pairs once per
-//     call by a small kernel in front;
-//   * four warps fetch the scales of the weight rows and of the rows of x (cp.async);
+//     call by a small kernel in front; it also fetches the scales of the weight rows and of the rows of x (cp.async);
 //   * two warps issue the MMAs of the even and the odd groups into two accumulators;
 //   * eight warps drain the accumulators: C[m, n] = fmaf(float(I), ws * asc, C) in registers, then the epilogue.
 #include <cuda.h>
@@ -36,10 +35,10 @@ constexpr int BP = 6;                               // stages of packed weights
 constexpr int SLOTS = 8;                            // stages of scales (reuse distance: see the loaders)
 constexpr int kLag = 2;                             // steps between issuing a fetch of scales and publishing it
 constexpr int B_BYTES = kCols * 256, BP_BYTES = 128 * 64;
-constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 3, SCALE_WARP0 = 4, EXP_WARP0 = 8, EPI_WARP0 = 16, kThreads = 24 * 32;
-// 768 threads start with 80 registers each (61 440 of the file); the shares below add up to the same
-constexpr int kRegsIssue = 48, kRegsScale = 40, kRegsExpand = 72, kRegsEpilogue = 120;
-static_assert(kRegsIssue + kRegsScale + 2 * kRegsExpand + 2 * kRegsEpilogue <= 480, "register shares of the six warpgroups");
+constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 3, EXP_WARP0 = 4, EPI_WARP0 = 12, kThreads = 20 * 32;
+// 640 threads start with 96 registers each (61 440 of the file); the shares below add up to no more
+constexpr int kRegsIssue = 72, kRegsExpand = 72, kRegsEpilogue = 128;
+static_assert(kRegsIssue + 2 * kRegsExpand + 2 * kRegsEpilogue <= 480, "register shares of the five warpgroups");
 static_assert(SLOTS >= RING + 2, "a scale slot is rewritten RING steps ahead of the MMAs, which are 2 ahead of the epilogue");
 constexpr int kSpin = 1 << 17;
 constexpr uint32_t kTmemCols = 512, kTmemA = 256;   // accumulators: columns 0..255; A: 4 x 64 columns
@@ -175,7 +174,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         }
         for (int i = 0; i < RING; i++) {
             mbar_init(&ctl->a_full[i], 4);
-            mbar_init(&ctl->b_full[i], 5);
+            mbar_init(&ctl->b_full[i], 2);
             mbar_init(&ctl->done[i], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -193,7 +192,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
     pdl_wait();
     const int total = count_units(p, kCols, tiles, ends, &bk);
 
-    if (warp < SCALE_WARP0) {
+    if (warp < EXP_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         // In these roles the whole warp walks the steps and one lane is elected to issue: a single lane that waits alone polls
         // its barrier dozens of times a step, and descriptors stay in uniform registers.
@@ -219,15 +218,30 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 for (int j = it > BP ? it - BP : 0; j < it; j++)
                     for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->bp_full[j % BP], (j / BP) & 1); i++) {}
         } else if (warp == ROW_WARP) {
-            // ================================================================ rows of x
+            // ================================================================ rows of x and all scales
             // A count of rows is a sum of boxes of 128, 64, 32 and 16: a box costs its issue, about 100 clocks, whatever it holds
-            // (16-row boxes throughout, 16 instructions a step, bound the tile at 1800 clocks; four-row gathers at 6000)
-            Ring<RING> r;
+            // (16-row boxes throughout, 16 instructions a step, bound the tile at 1800 clocks; four-row gathers at 6000).
+            // A lane fetches the scales of four rows of x and the aligned words around those of four weight rows (a copy has at
+            // least four bytes; allocations are whole words).  Slot it % SLOTS was last read by the epilogue of step it - SLOTS:
+            // stage it % RING is free when the MMAs of step it - RING have run, which were issued after the accumulator of step
+            // it - RING - 2 had been drained.
+            Ring<RING> r, behind;
+            const uint32_t sdst0 = smem_u32(sring) + lane * 4, wdst0 = smem_u32(wsring) + lane * 4;
             int it = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const int n16 = (un.count + 15) & ~15;
+                const float* sc[4];
+                uintptr_t wsc[4];
+                bool has[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const long long sr = x_row(p, un, lane + 32 * i);
+                    has[i] = sr >= 0;
+                    sc[i] = p.asc + (sr < 0 ? 0 : (size_t)sr * G);
+                    wsc[i] = reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, lane + 32 * i) * G);
+                }
                 for (int g = 0; g < G; g++, it++, r.next()) {
                     if (it >= RING && !(ok = wait_warp(&ctl->done[r.s], r.ph ^ 1, ctl, 25))) break;
                     uint64_t* bar = &ctl->b_full[r.s];
@@ -244,8 +258,27 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                             }
                     }
                     __syncwarp();
+                    const uint32_t slot = (it % SLOTS) * 512;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        cp_async4(sdst0 + slot + 128 * i, sc[i], has[i]);
+                        cp_async4(wdst0 + slot + 128 * i, reinterpret_cast<const void*>(wsc[i] & ~(uintptr_t)3), true);
+                        sc[i]++;
+                        wsc[i] += 2;
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (it >= kLag) {
+                        cp_async_wait<kLag>();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&ctl->b_full[behind.s]);
+                        behind.next();
+                    }
                 }
             }
+            cp_async_wait<0>();
+            __syncwarp();
+            if (ok && lane == 0)
+                for (int j = it > kLag ? it - kLag : 0; j < it; j++, behind.next()) mbar_arrive(&ctl->b_full[behind.s]);
             if (ctl->abort)
                 for (int j = it > RING ? it - RING : 0; j < it; j++)
                     for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->b_full[j % RING], (j / RING) & 1); i++) {}
@@ -281,40 +314,6 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             if (elect_one()) tc_commit(&ctl->drain[par]);
             for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->drain[par], 0); i++) {}
         }
-    } else if (warp < EXP_WARP0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsScale));
-        // ==================================================================== scales
-        // Thread i fetches the scale of row i of x and the aligned word around that of weight row i (a copy has at least four
-        // bytes; allocations are whole words).  Slot it % SLOTS was last read by the epilogue of step it - SLOTS: stage
-        // it % RING is free when the MMAs of step it - RING have run, which were issued after the accumulator of step
-        // it - RING - 2 had been drained.
-        const int i = threadIdx.x - SCALE_WARP0 * 32;
-        const uint32_t sdst0 = smem_u32(sring) + i * 4, wdst0 = smem_u32(wsring) + i * 4;
-        Ring<RING> r, behind;
-        int it = 0;
-        bool ok = true;
-        for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
-            const Unit un = find_unit(p, u, kCols, tiles, ends);
-            const long long sr = x_row(p, un, i);
-            const float* sc = p.asc + (sr < 0 ? 0 : (size_t)sr * G);
-            const __half* wsc = p.ws + weight_row<GATED>(p, un, i) * G;
-            for (int g = 0; g < G; g++, it++, r.next()) {
-                if (it >= RING && !(ok = wait_warp(&ctl->done[r.s], r.ph ^ 1, ctl, 29))) break;
-                cp_async4(sdst0 + (it % SLOTS) * (kCols * 4), sc + g, sr >= 0);
-                cp_async4(wdst0 + (it % SLOTS) * 512, reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(wsc + g) & ~(uintptr_t)3), true);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                if (it >= kLag) {
-                    cp_async_wait<kLag>();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&ctl->b_full[behind.s]);
-                    behind.next();
-                }
-            }
-        }
-        cp_async_wait<0>();
-        __syncwarp();
-        if (ok && lane == 0)
-            for (int j = it > kLag ? it - kLag : 0; j < it; j++, behind.next()) mbar_arrive(&ctl->b_full[behind.s]);
     } else if (warp < EPI_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsExpand));
         // ==================================================================== expansion of the weights

@@ -16,7 +16,7 @@ import dataclasses
 import numpy as np
 
 from .model import Workspace, _as_rows
-from .runtime import Runtime
+from .runtime import Runtime, _bits
 
 __all__ = ["ACTIVATIONS", "FusedLinear", "MoEPlan", "MoERouter", "ExpertLinear", "MoEMLP"]
 
@@ -158,18 +158,26 @@ class MoERouter:
             if bias.shape != (self.n_exp,):
                 raise ValueError(f"bias {bias.shape} does not match the {self.n_exp} experts")
             self.bias = self.ws.upload(self.tag + ".bias", bias)
-        self._tail = (int(n_group), int(topk_group), int(group_top), SCORES[score], int(bool(renorm)), float(scale),
+        self._key, self._last = self.tag + ".plan", None
+        self._tail = (int(n_group), int(topk_group), int(group_top), SCORES[score], int(bool(renorm)), _bits(float(scale)),
                       LOGIT_TYPES[dtype])
 
     def forward_device(self, logits_dev: int, rows: int, sync: bool = False) -> MoEPlan:
         """Queues the routing; the plan's buffers belong to the router and hold until its next call."""
         if rows < 0:
             raise ValueError(f"rows={rows}")
-        pairs4 = max(1, rows * self.topk) * 4
-        b = {n: self.ws.buffer(f"{self.tag}.{n}", pairs4) for n in ("ids", "weights", "bucket_rows", "base")}
-        plan = MoEPlan(rows, self.topk, self.n_exp, offsets=self.ws.buffer(self.tag + ".offsets", (self.n_exp + 1) * 4), **b)
-        self.rt.launch("moe_route_plan_k", 1, 1, [int(logits_dev), self.bias, plan.ids, plan.weights, plan.bucket_rows, plan.base,
-                                                  plan.offsets, rows, self.n_exp, self.topk, *self._tail])
+        # plan and arguments of the last call are used again while the row count and the block of memory are the same
+        if self._last is None or self._last[0] != rows or self.ws._bufs.get(self._key) is not self._last[1]:
+            array = -(-max(1, rows * self.topk) * 4 // 256) * 256
+            at = self.ws.buffer(self._key, 4 * array + (self.n_exp + 1) * 4)
+            plan = MoEPlan(rows, self.topk, self.n_exp, ids=at, weights=at + array, bucket_rows=at + 2 * array, base=at + 3 * array,
+                           offsets=at + 4 * array)
+            self._last = (rows, self.ws._bufs[self._key], plan,
+                          [0, self.bias, plan.ids, plan.weights, plan.bucket_rows, plan.base, plan.offsets, rows, self.n_exp,
+                           self.topk, *self._tail])
+        plan, argv = self._last[2:]
+        argv[0] = int(logits_dev)
+        self.rt.launch("moe_route_plan_k", 1, 1, argv)
         if sync:
             self.rt.sync()
         return plan
