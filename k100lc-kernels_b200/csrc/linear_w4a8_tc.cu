@@ -53,9 +53,9 @@ struct __align__(16) Control {
 
 __device__ int g_status;                            // 0, or the code 21.. of the first bounded wait that ran out
 
-__device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity, Control* ctl, int code) {
+__device__ __forceinline__ bool wait(uint32_t b, uint32_t parity, Control* ctl, int code) {
     for (int i = 0; i < kSpin; i++) {
-        if (mbar_try_wait(b, parity)) return true;
+        if (mbar_try_wait_at(b, parity)) return true;
         if ((i & 63) == 63 && ctl->abort) return false;
     }
     ctl->abort = 1;
@@ -63,8 +63,8 @@ __device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity, Control* ctl,
     return false;
 }
 // the same by all lanes of a warp, which leave it with one answer (their next instructions are warp-wide)
-__device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, Control* ctl, int code) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return true;
+__device__ __forceinline__ bool wait_warp(uint32_t b, uint32_t parity, Control* ctl, int code) {
+    if (__all_sync(0xffffffffu, mbar_try_wait_at(b, parity))) return true;
     return __all_sync(0xffffffffu, wait(b, parity, ctl, code));
 }
 
@@ -134,18 +134,21 @@ __device__ __forceinline__ size_t weight_row(const Params& p, const Unit& u, int
     return (size_t)u.expert * 2 * p.N + (row < 64 ? 0 : p.N) + min(u.tile * 64 + (row & 63), p.N - 1);
 }
 
-// Position in a ring of N stages and the parity of its phase there.
+// Position in a ring of N stages and the parity of its phase there.  A wait for the other parity passes at once in the first
+// round: the phase before a barrier's first counts as complete.
 template <int N>
 struct Ring {
-    int s = 0;
-    uint32_t ph = 0;
+    uint32_t s = 0, ph = 0;
     __device__ __forceinline__ void next() {
-        if (++s == N) {
-            s = 0;
-            ph ^= 1;
-        }
+        s = s + 1 == N ? 0 : s + 1;
+        ph ^= s == 0 ? 1u : 0u;
+    }
+    __device__ __forceinline__ void next2() {                         // two steps on; N is even
+        s = s + 2 >= N ? s + 2 - N : s + 2;
+        ph ^= s < 2 ? 1u : 0u;
     }
 };
+static_assert(RING % 2 == 0 && BP % 2 == 0 && SLOTS == 2 * RING, "even and odd steps have stages, accumulators and slots of their own");
 
 struct RowMaps { CUtensorMap box[4]; };             // boxes of 128, 64, 32 and 16 rows of x (64 k)
 
@@ -192,6 +195,9 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
     pdl_wait();
     const int total = count_units(p, kCols, tiles, ends, &bk);
 
+    const uint32_t bring_s = smem_u32(bring), wring_s = smem_u32(wring), sring_s = smem_u32(sring), wsring_s = smem_u32(wsring);
+    const uint32_t bp_full = smem_u32(ctl->bp_full), bp_free = smem_u32(ctl->bp_free), a_full = smem_u32(ctl->a_full), b_full = smem_u32(ctl->b_full);
+    const uint32_t done = smem_u32(ctl->done), acc_free = smem_u32(ctl->acc_free);
     if (warp < EXP_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         // In these roles the whole warp walks the steps and one lane is elected to issue: a single lane that waits alone polls
@@ -205,11 +211,12 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const int y0 = un.expert * (GATED ? 2 * p.N : p.N) + un.tile * ROWS, y1 = y0 + (GATED ? p.N : 64);
                 for (int g = 0; g < G; g++, it++, r.next()) {
-                    if (it >= BP && !(ok = wait_warp(&ctl->bp_free[r.s], r.ph ^ 1, ctl, 21))) break;
+                    if (!(ok = wait_warp(bp_free + r.s * 8, r.ph ^ 1, ctl, 21))) break;
                     if (elect_one()) {
-                        mbar_expect_tx(&ctl->bp_full[r.s], BP_BYTES);
-                        tma_2d(wring + r.s * BP_BYTES, &map_w, g * 64, y0, &ctl->bp_full[r.s]);
-                        tma_2d(wring + r.s * BP_BYTES + BP_BYTES / 2, &map_w, g * 64, y1, &ctl->bp_full[r.s]);
+                        const uint32_t bar = bp_full + r.s * 8, dst = wring_s + r.s * BP_BYTES;
+                        mbar_expect_tx_at(bar, BP_BYTES);
+                        tma_2d_at(dst, &map_w, g * 64, y0, bar);
+                        tma_2d_at(dst + BP_BYTES / 2, &map_w, g * 64, y1, bar);
                     }
                     __syncwarp();
                 }
@@ -226,7 +233,6 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             // stage it % RING is free when the MMAs of step it - RING have run, which were issued after the accumulator of step
             // it - RING - 2 had been drained.
             Ring<RING> r, behind;
-            const uint32_t sdst0 = smem_u32(sring) + lane * 4, wdst0 = smem_u32(wsring) + lane * 4;
             int it = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
@@ -243,26 +249,27 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                     wsc[i] = reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, lane + 32 * i) * G);
                 }
                 for (int g = 0; g < G; g++, it++, r.next()) {
-                    if (it >= RING && !(ok = wait_warp(&ctl->done[r.s], r.ph ^ 1, ctl, 25))) break;
-                    uint64_t* bar = &ctl->b_full[r.s];
+                    if (!(ok = wait_warp(done + r.s * 8, r.ph ^ 1, ctl, 25))) break;
                     if (elect_one()) {
-                        mbar_expect_tx(bar, (uint32_t)n16 * 256);
-                        uint8_t* dst = bring + r.s * B_BYTES;
-                        int at = 0;
+                        const uint32_t bar = b_full + r.s * 8;
+                        mbar_expect_tx_at(bar, (uint32_t)n16 * 256);
+                        uint32_t dst = bring_s + r.s * B_BYTES;
+                        int at = un.first;
 #pragma unroll
                         for (int b = 0; b < 4; b++)
                             if (n16 & (128 >> b)) {
-                                tma_2d(dst + at * 128, &map_x.box[b], g * 256, un.first + at, bar);
-                                tma_2d(dst + at * 128 + kCols * 128, &map_x.box[b], g * 256 + 128, un.first + at, bar);
+                                tma_2d_at(dst, &map_x.box[b], g * 256, at, bar);
+                                tma_2d_at(dst + kCols * 128, &map_x.box[b], g * 256 + 128, at, bar);
                                 at += 128 >> b;
+                                dst += (128 >> b) * 128;
                             }
                     }
                     __syncwarp();
-                    const uint32_t slot = (it % SLOTS) * 512;
+                    const uint32_t slot = (r.s + RING * r.ph) * 512 + lane * 4;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        cp_async4(sdst0 + slot + 128 * i, sc[i], has[i]);
-                        cp_async4(wdst0 + slot + 128 * i, reinterpret_cast<const void*>(wsc[i] & ~(uintptr_t)3), true);
+                        cp_async4(sring_s + slot + 128 * i, sc[i], has[i]);
+                        cp_async4(wsring_s + slot + 128 * i, reinterpret_cast<const void*>(wsc[i] & ~(uintptr_t)3), true);
                         sc[i]++;
                         wsc[i] += 2;
                     }
@@ -270,7 +277,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                     if (it >= kLag) {
                         cp_async_wait<kLag>();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&ctl->b_full[behind.s]);
+                        if (lane == 0) mbar_arrive_at(b_full + behind.s * 8);
                         behind.next();
                     }
                 }
@@ -278,25 +285,26 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             cp_async_wait<0>();
             __syncwarp();
             if (ok && lane == 0)
-                for (int j = it > kLag ? it - kLag : 0; j < it; j++, behind.next()) mbar_arrive(&ctl->b_full[behind.s]);
+                for (int j = it > kLag ? it - kLag : 0; j < it; j++, behind.next()) mbar_arrive_at(b_full + behind.s * 8);
             if (ctl->abort)
                 for (int j = it > RING ? it - RING : 0; j < it; j++)
                     for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->b_full[j % RING], (j / RING) & 1); i++) {}
         } else {
             // ================================================================ MMA issuers: even and odd steps
-            const int par = warp - MMA_WARP;
-            const uint64_t bdesc0 = smem_desc_sw128(smem_u32(bring));
+            const uint32_t par = warp - MMA_WARP;
+            const uint64_t bdesc0 = smem_desc_sw128(bring_s);
             Ring<RING> r;
-            int it = 0;
+            uint32_t parity = 0;                                     // of the first step of the tile
+            if (par) r.next();
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const uint32_t idesc = instr_desc((un.count + 15) & ~15);
-                for (int g = 0; g < G; g++, it++, r.next()) {
-                    if ((it & 1) != par) continue;
-                    if (!(ok = wait_warp(&ctl->a_full[r.s], r.ph, ctl, 23))) break;
-                    if (!(ok = wait_warp(&ctl->b_full[r.s], r.ph, ctl, 24))) break;
-                    if (it >= 2 && !(ok = wait_warp(&ctl->acc_free[par], ((it >> 1) & 1) ^ 1, ctl, 22))) break;
+                for (int g = par ^ parity; g < G; g += 2, r.next2()) {
+                    if (!(ok = wait_warp(a_full + r.s * 8, r.ph, ctl, 23))) break;
+                    if (!(ok = wait_warp(b_full + r.s * 8, r.ph, ctl, 24))) break;
+                    // (an accumulator's phase is over every second step: s / 2 and the ring's phase count them)
+                    if (!(ok = wait_warp(acc_free + par * 8, (r.s >> 1) ^ 1, ctl, 22))) break;
                     tc_fence_after();
                     const uint64_t bd = bdesc0 + (uint64_t)(r.s * (B_BYTES >> 4));
                     const uint32_t d = tmem + par * kCols, a = tmem + kTmemA + r.s * 64;
@@ -304,10 +312,11 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 #pragma unroll
                         for (int j = 0; j < 8; j++)                  // 16 k each: 8 columns of A, 32 bytes of B
                             tc_mma_f16_ts(d, a + j * 8, bd + (j >> 2) * (kCols * 128 >> 4) + (j & 3) * 2, idesc, j > 0);
-                        tc_commit(&ctl->done[r.s]);
+                        tc_commit_at(done + r.s * 8);
                     }
                     __syncwarp();
                 }
+                parity ^= G & 1;
             }
             // nothing this warp issued may still run when tensor memory is released (the lane that issued commits: elect.sync
             // names the same lane of a full warp every time)
@@ -316,25 +325,25 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         }
     } else if (warp < EPI_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsExpand));
-        // ==================================================================== expansion of the weights
-        const int set = (warp - EXP_WARP0) >> 2, q = warp & 3, row = q * 32 + lane;
+        // ==================================================================== expansion of the weights: even and odd steps
+        const uint32_t set = (warp - EXP_WARP0) >> 2, q = warp & 3, row = q * 32 + lane;
         const uint32_t a0 = tmem + ((uint32_t)(q * 32) << 16) + kTmemA;
-        const uint8_t* w0 = wring + row * 64;
-        const int x = ((row >> 1) & 3) << 4;                         // 64-byte swizzle: chunk ^= (row / 2) % 4
+        const uint32_t x = ((row >> 1) & 3) << 4;                    // 64-byte swizzle: chunk ^= (row / 2) % 4
+        const uint32_t w0 = wring_s + row * 64 + x, w1 = wring_s + row * 64 + (16 ^ x), w2 = wring_s + row * 64 + (32 ^ x), w3 = wring_s + row * 64 + (48 ^ x);
         Ring<BP> rp;
         Ring<RING> r;
-        int it = 0;
+        uint32_t parity = 0;
+        if (set) {
+            rp.next();
+            r.next();
+        }
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
-            for (int g = 0; g < G; g++, it++, rp.next(), r.next()) {
-                if ((it & 1) != set) continue;
-                if (!(ok = wait_warp(&ctl->bp_full[rp.s], rp.ph, ctl, 26))) break;
-                uint4 w[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) w[j] = *reinterpret_cast<const uint4*>(w0 + rp.s * BP_BYTES + ((j << 4) ^ x));
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->bp_free[rp.s]);
-                if (it >= RING && !(ok = wait_warp(&ctl->done[r.s], r.ph ^ 1, ctl, 27))) break;
+            for (int g = set ^ parity; g < G; g += 2, rp.next2(), r.next2()) {
+                if (!(ok = wait_warp(bp_full + rp.s * 8, rp.ph, ctl, 26))) break;
+                const uint32_t at = rp.s * BP_BYTES;
+                const uint4 w[4] = {lds128(w0 + at), lds128(w1 + at), lds128(w2 + at), lds128(w3 + at)};
+                if (!(ok = wait_warp(done + r.s * 8, r.ph ^ 1, ctl, 27))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -351,35 +360,37 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 }
                 tmem_st_wait();
                 tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->a_full[r.s]);
+                __syncwarp();                                        // (every lane has its words in registers, and A is written)
+                if (lane == 0) {
+                    mbar_arrive_at(bp_free + rp.s * 8);
+                    mbar_arrive_at(a_full + r.s * 8);
+                }
             }
+            parity ^= G & 1;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
         // ==================================================================== epilogue
         // warp: lanes 32 q .. of the accumulators, 16-column chunks half, half + 2, ... of the tile
         const int q = warp & 3, half = (warp - EPI_WARP0) >> 2, row = q * 32 + lane;
-        const uint32_t d0 = tmem + ((uint32_t)(q * 32) << 16) + half * 16;
+        const uint32_t d0 = tmem + ((uint32_t)(q * 32) << 16) + half * 16, sb0 = sring_s + half * 64, sw0 = wsring_s + row * 4;
         Ring<RING> r;
-        int it = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
             const Unit un = find_unit(p, u, kCols, tiles, ends);
             const int n0 = un.tile * ROWS, chunks = (un.count - half * 16 + 31) >> 5;
-            uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, row) * G) >> 1) & 1;   // half of the word
+            // which half of its word the scale of group g is: by g's parity
+            uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, row) * G) >> 1) << 4 & 16;
             uint64_t C[4][8];                                        // pairs of neighbouring columns
 #pragma unroll
             for (int a = 0; a < 4; a++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) C[a][j] = 0;
-            for (int g = 0; g < G; g++, it++, odd ^= 1, r.next()) {
-                const float* sb = sring + (it % SLOTS) * kCols + half * 16;
-                if (!(ok = wait_warp(&ctl->done[r.s], r.ph, ctl, 28))) break;
+            for (int g = 0; g < G; g++, shift ^= 16, r.next()) {
+                if (!(ok = wait_warp(done + r.s * 8, r.ph, ctl, 28))) break;
                 tc_fence_after();
-                const uint32_t d = d0 + (it & 1) * kCols;
-                const uint32_t sw = wsring[(it % SLOTS) * 128 + row];
-                const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(odd ? sw >> 16 : sw & 0xffffu))));
+                const uint32_t slot = (r.s + RING * r.ph) * 512, sb = sb0 + slot, d = d0 + (r.s & 1) * kCols;
+                const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(lds32(sw0 + slot) >> shift))));
                 const uint64_t s2 = pack2(s, s);
 #pragma unroll
                 for (int a = 0; a < 4; a++) {
@@ -387,9 +398,9 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                     uint64_t f[8], v[8];
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
-                        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sb + a * 32 + 2 * j);
-                        f[j] = mul2p(s2, b.x);
-                        f[j + 1] = mul2p(s2, b.y);
+                        const uint4 b = lds128(sb + a * 128 + j * 8);
+                        f[j] = mul2p(s2, pack2(b.x, b.y));
+                        f[j + 1] = mul2p(s2, pack2(b.z, b.w));
                     }
                     tmem_ld16_pairs(d + a * 32, v);
 #pragma unroll
@@ -397,12 +408,12 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->acc_free[it & 1]);
+                if (lane == 0) mbar_arrive_at(acc_free + (r.s & 1) * 8);
             }
             if (!ok) break;
+            const float bias = p.bias ? p.bias[weight_row<GATED>(p, un, row)] : 0.f;
             // 32 columns at a time through shared memory, so that the loop with the activation stays rolled: unrolled over
             // the registers it was 60 KB of code, and fetching that took 1.7 times as long as the tile's products
-            const float bias = p.bias ? p.bias[weight_row<GATED>(p, un, row)] : 0.f;
 #pragma unroll
             for (int a = 0; a < 4; a++) {
                 if (a * 32 >= un.count) break;
