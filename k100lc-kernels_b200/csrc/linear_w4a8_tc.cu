@@ -3,19 +3,18 @@
 //
 // D^T[weight row][row of x] = W . x^T: 128 weight rows (gated: 64 gate rows and the 64 up rows beside them) are the 128
 // lanes of an accumulator, up to 128 rows of a bucket its columns, so that a short bucket costs a narrow MMA and not a
-// padded tile.  The product of a 128-group is one exact integer, formed as a float: int4 weights and int8 codes are
-// exact in f16, a product is below 2^10, a sum of 128 below 2^17, so tcgen05.mma.kind::f16 with fp32 accumulators
-// returns float(I) and the epilogue needs no conversion (with kind::i8 the conversions, 16 a clock per SM, take four
-// times as long as the MMAs).
+// padded tile.  tcgen05.mma.kind::i8 forms the exact integer of a 128-group; the weights enter as 16 w, a nibble in the
+// upper half of its byte, which takes two logic instructions for eight of them, and the 16 is divided out of their scale.
+// (kind::f16, whose fp32 accumulators need no conversion, was a third slower: its expansion takes nine instructions for
+// eight weights, its rows of x twice the bytes, and its MMAs leave tensor memory for two accumulators instead of three.)
 //
 // Roles of the 20 warps of the persistent CTA, joined by mbarriers (every wait is bounded):
 //   * one warp copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring;
-//   * eight warps expand them: a thread owns a weight row, reads its 64 bytes, turns nibbles into f16 pairs with four
-//     logic and four arithmetic instructions a word, and writes them to tensor memory, from where the MMA takes its A
-//     operand: no shared-memory traffic for the wide operand, which would otherwise bound the tile (128 bytes a clock);
-//   * one warp copies the rows of x by TMA: f16, put into bucket order and into the k order of the nibble pairs once per
-//     call by a small kernel in front; it also fetches the scales of the weight rows and of the rows of x (cp.async);
-//   * two warps issue the MMAs of the even and the odd groups into two accumulators;
+//   * eight warps expand them: a thread owns a weight row, reads its 64 bytes and writes 128 to tensor memory, from where
+//     the MMA takes its A operand;
+//   * one warp copies the rows of x by TMA, put into bucket order and into the k order of the nibbles once per call by a
+//     small kernel in front; it also fetches the scales of the weight rows and of the rows of x (cp.async);
+//   * two warps issue the MMAs of the even and the odd groups, into three accumulators in turn;
 //   * eight warps drain the accumulators: C[m, n] = fmaf(float(I), ws * asc, C) in registers, then the epilogue.
 #include <cuda.h>
 
@@ -31,22 +30,24 @@ using namespace tc;
 
 constexpr int kCols = 128;                          // rows of x per tile
 constexpr int RING = 4;                             // stages of A (tensor memory), B (shared memory) and "step done" barriers
-constexpr int BP = 6;                               // stages of packed weights
-constexpr int SLOTS = 8;                            // stages of scales (reuse distance: see the loaders)
+constexpr int NACC = 3;                             // accumulators
+constexpr int BP = 8;                               // stages of packed weights
+constexpr int SLOTS = 8;                            // stages of scales (reuse distance: see where they are fetched)
 constexpr int kLag = 2;                             // steps between issuing a fetch of scales and publishing it
-constexpr int B_BYTES = kCols * 256, BP_BYTES = 128 * 64;
+constexpr int B_BYTES = kCols * 128, BP_BYTES = 128 * 64;
 constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 3, EXP_WARP0 = 4, EPI_WARP0 = 12, kThreads = 20 * 32;
 // 640 threads start with 96 registers each (61 440 of the file); the shares below add up to no more
 constexpr int kRegsIssue = 72, kRegsExpand = 72, kRegsEpilogue = 128;
 static_assert(kRegsIssue + 2 * kRegsExpand + 2 * kRegsEpilogue <= 480, "register shares of the five warpgroups");
-static_assert(SLOTS >= RING + 2, "a scale slot is rewritten RING steps ahead of the MMAs, which are 2 ahead of the epilogue");
+static_assert(SLOTS >= RING + NACC, "a scale slot is rewritten RING steps ahead of the MMAs, which are NACC ahead of the epilogue");
 constexpr int kSpin = 1 << 17;
-constexpr uint32_t kTmemCols = 512, kTmemA = 256;   // accumulators: columns 0..255; A: 4 x 64 columns
+constexpr uint32_t kTmemCols = 512, kTmemA = NACC * kCols;   // accumulators, then A: 4 x 32 columns
+static_assert(NACC * kCols + RING * 32 <= 512, "tensor memory");
 
 struct __align__(16) Control {
     uint64_t bp_full[BP], bp_free[BP];
     uint64_t a_full[RING], b_full[RING], done[RING];
-    uint64_t acc_free[2], drain[2];
+    uint64_t acc_free[NACC], drain[2];
     uint32_t tmem_base;
     volatile int abort;
 };
@@ -68,35 +69,21 @@ __device__ __forceinline__ bool wait_warp(uint32_t b, uint32_t parity, Control* 
     return __all_sync(0xffffffffu, wait(b, parity, ctl, code));
 }
 
-// kind::f16: f32 accumulator, f16 operands, both K-major, M = 128
-__device__ __forceinline__ uint32_t instr_desc(int n) { return 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24; }
+// kind::i8: s32 accumulator, s8 operands, both K-major, M = 128
+__device__ __forceinline__ uint32_t instr_desc(int n) { return 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24; }
 
-// Eight two's-complement nibbles of a word -> four f16 pairs (k0,k4) (k1,k5) (k2,k6) (k3,k7), exact: 0x6400 is 1024 with
-// steps of 1, so nibble ^ 8 in the low bits is 1024 + u, and in the next four bits 1024 + 16 u.
-__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
+// Eight two's-complement nibbles of a word -> 16 times their value as bytes, k0,k2,k4,k6 and k1,k3,k5,k7.
 __device__ __forceinline__ void expand_word(uint32_t w, uint32_t* o) {
-    const uint32_t v = w >> 8;
-    o[0] = sub_f16x2((w & 0x000F000Fu) ^ 0x64086408u, 0x64086408u);                          // - 1032
-    o[1] = fma_f16x2((w & 0x00F000F0u) ^ 0x64806480u, 0x2C002C00u, 0xD480D480u);             // / 16 - 72
-    o[2] = sub_f16x2((v & 0x000F000Fu) ^ 0x64086408u, 0x64086408u);
-    o[3] = fma_f16x2((v & 0x00F000F0u) ^ 0x64806480u, 0x2C002C00u, 0xD480D480u);
+    o[0] = (w << 4) & 0xF0F0F0F0u;
+    o[1] = w & 0xF0F0F0F0u;
 }
 
-// codes [xrows][K/2] even and odd -> f16 [m][K] in the pair order above; slot s of a plan takes row bucket_rows[s].  A thread
-// turns 16 k; slots behind the last bucket and slots of no row are skipped.
+// codes [xrows][K/2] even and odd -> [m][K] in that order; slot s of a plan takes row bucket_rows[s].  A thread moves 32 k;
+// slots behind the last bucket and slots of no row are skipped.
 __global__ void __launch_bounds__(256)
-expand_codes_kernel(const Params p, __half* __restrict__ out) {
+order_codes_kernel(const Params p, int8_t* __restrict__ out) {
     pdl_wait();
-    const int per_row = p.K / 16;
+    const int per_row = p.K / 32;
     const long long used = p.offsets ? bound(p, p.n_exp) : p.m, n = used * per_row;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
         const long long slot = i / per_row;
@@ -106,18 +93,11 @@ expand_codes_kernel(const Params p, __half* __restrict__ out) {
             row = p.bucket_rows[slot];
             if (row < 0 || row >= p.xrows) continue;
         }
-        const uint2 e = *reinterpret_cast<const uint2*>(p.ae + row * (p.K / 2) + c * 8);
-        const uint2 o = *reinterpret_cast<const uint2*>(p.ao + row * (p.K / 2) + c * 8);
-        uint4* dst = reinterpret_cast<uint4*>(out + slot * p.K + c * 16);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const uint32_t a = h ? e.y : e.x, b = h ? o.y : o.x;
-            auto pair = [](uint32_t w, int j) {                      // bytes j and j + 2
-                const __half2 v = __floats2half2_rn((float)(int8_t)(w >> (8 * j)), (float)(int8_t)(w >> (8 * j + 16)));
-                return *reinterpret_cast<const uint32_t*>(&v);
-            };
-            dst[h] = make_uint4(pair(a, 0), pair(b, 0), pair(a, 1), pair(b, 1));
-        }
+        const uint4 e = *reinterpret_cast<const uint4*>(p.ae + row * (p.K / 2) + c * 16);
+        const uint4 o = *reinterpret_cast<const uint4*>(p.ao + row * (p.K / 2) + c * 16);
+        uint4* dst = reinterpret_cast<uint4*>(out + slot * p.K + c * 32);
+        dst[0] = make_uint4(e.x, o.x, e.y, o.y);
+        dst[1] = make_uint4(e.z, o.z, e.w, o.w);
     }
     pdl_launch_dependents();
 }
@@ -143,14 +123,14 @@ struct Ring {
         s = s + 1 == N ? 0 : s + 1;
         ph ^= s == 0 ? 1u : 0u;
     }
-    __device__ __forceinline__ void next2() {                         // two steps on; N is even
+    __device__ __forceinline__ void next2() {                         // two steps on
         s = s + 2 >= N ? s + 2 - N : s + 2;
         ph ^= s < 2 ? 1u : 0u;
     }
 };
-static_assert(RING % 2 == 0 && BP % 2 == 0 && SLOTS == 2 * RING, "even and odd steps have stages, accumulators and slots of their own");
+static_assert(SLOTS == 2 * RING, "a ring position and its phase name a slot");
 
-struct RowMaps { CUtensorMap box[4]; };             // boxes of 128, 64, 32 and 16 rows of x (64 k)
+struct RowMaps { CUtensorMap box[4]; };             // boxes of 128, 64, 32 and 16 rows of x (a group)
 
 // GATED: 64 gate rows and 64 up rows make a tile.
 template <bool GATED>
@@ -158,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ RowMaps map_x, const Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t* bring = smem;                                           // RING x [2 halves of 64 k][128 rows][128 bytes]
+    uint8_t* bring = smem;                                           // RING x [128 rows][128 bytes]
     uint8_t* wring = bring + RING * B_BYTES;                         // BP x [128 rows][64 bytes]
     float* sring = reinterpret_cast<float*>(wring + BP * BP_BYTES);  // SLOTS x [128]
     uint32_t* wsring = reinterpret_cast<uint32_t*>(sring + SLOTS * kCols);   // SLOTS x [128]: the word that holds the weight row's scale
@@ -180,10 +160,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             mbar_init(&ctl->b_full[i], 2);
             mbar_init(&ctl->done[i], 1);
         }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&ctl->acc_free[i], 8);
-            mbar_init(&ctl->drain[i], 1);
-        }
+        for (int i = 0; i < NACC; i++) mbar_init(&ctl->acc_free[i], 8);
+        for (int i = 0; i < 2; i++) mbar_init(&ctl->drain[i], 1);
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -231,7 +209,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             // A lane fetches the scales of four rows of x and the aligned words around those of four weight rows (a copy has at
             // least four bytes; allocations are whole words).  Slot it % SLOTS was last read by the epilogue of step it - SLOTS:
             // stage it % RING is free when the MMAs of step it - RING have run, which were issued after the accumulator of step
-            // it - RING - 2 had been drained.
+            // it - RING - NACC had been drained.
             Ring<RING> r, behind;
             int it = 0;
             bool ok = true;
@@ -252,14 +230,13 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                     if (!(ok = wait_warp(done + r.s * 8, r.ph ^ 1, ctl, 25))) break;
                     if (elect_one()) {
                         const uint32_t bar = b_full + r.s * 8;
-                        mbar_expect_tx_at(bar, (uint32_t)n16 * 256);
+                        mbar_expect_tx_at(bar, (uint32_t)n16 * 128);
                         uint32_t dst = bring_s + r.s * B_BYTES;
                         int at = un.first;
 #pragma unroll
                         for (int b = 0; b < 4; b++)
                             if (n16 & (128 >> b)) {
-                                tma_2d_at(dst, &map_x.box[b], g * 256, at, bar);
-                                tma_2d_at(dst + kCols * 128, &map_x.box[b], g * 256 + 128, at, bar);
+                                tma_2d_at(dst, &map_x.box[b], g * 128, at, bar);
                                 at += 128 >> b;
                                 dst += (128 >> b) * 128;
                             }
@@ -294,24 +271,27 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             const uint32_t par = warp - MMA_WARP;
             const uint64_t bdesc0 = smem_desc_sw128(bring_s);
             Ring<RING> r;
+            Ring<NACC> acc;
             uint32_t parity = 0;                                     // of the first step of the tile
-            if (par) r.next();
+            if (par) {
+                r.next();
+                acc.next();
+            }
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const uint32_t idesc = instr_desc((un.count + 15) & ~15);
-                for (int g = par ^ parity; g < G; g += 2, r.next2()) {
+                for (int g = par ^ parity; g < G; g += 2, r.next2(), acc.next2()) {
                     if (!(ok = wait_warp(a_full + r.s * 8, r.ph, ctl, 23))) break;
                     if (!(ok = wait_warp(b_full + r.s * 8, r.ph, ctl, 24))) break;
-                    // (an accumulator's phase is over every second step: s / 2 and the ring's phase count them)
-                    if (!(ok = wait_warp(acc_free + par * 8, (r.s >> 1) ^ 1, ctl, 22))) break;
+                    if (!(ok = wait_warp(acc_free + acc.s * 8, acc.ph ^ 1, ctl, 22))) break;
                     tc_fence_after();
                     const uint64_t bd = bdesc0 + (uint64_t)(r.s * (B_BYTES >> 4));
-                    const uint32_t d = tmem + par * kCols, a = tmem + kTmemA + r.s * 64;
+                    const uint32_t d = tmem + acc.s * kCols, a = tmem + kTmemA + r.s * 32;
                     if (elect_one()) {
 #pragma unroll
-                        for (int j = 0; j < 8; j++)                  // 16 k each: 8 columns of A, 32 bytes of B
-                            tc_mma_f16_ts(d, a + j * 8, bd + (j >> 2) * (kCols * 128 >> 4) + (j & 3) * 2, idesc, j > 0);
+                        for (int j = 0; j < 4; j++)                  // 32 k each: 8 columns of A, 32 bytes of B
+                            tc_mma_i8_ts(d, a + j * 8, bd + j * 2, idesc, j > 0);
                         tc_commit_at(done + r.s * 8);
                     }
                     __syncwarp();
@@ -345,19 +325,15 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 const uint4 w[4] = {lds128(w0 + at), lds128(w1 + at), lds128(w2 + at), lds128(w3 + at)};
                 if (!(ok = wait_warp(done + r.s * 8, r.ph ^ 1, ctl, 27))) break;
                 tc_fence_after();
+                uint32_t o[32];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t o[32];
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const uint4 v = w[2 * h + j];
-                        expand_word(v.x, o + 16 * j);
-                        expand_word(v.y, o + 16 * j + 4);
-                        expand_word(v.z, o + 16 * j + 8);
-                        expand_word(v.w, o + 16 * j + 12);
-                    }
-                    tmem_st32(a0 + r.s * 64 + h * 32, o);
+                for (int j = 0; j < 4; j++) {
+                    expand_word(w[j].x, o + 8 * j);
+                    expand_word(w[j].y, o + 8 * j + 2);
+                    expand_word(w[j].z, o + 8 * j + 4);
+                    expand_word(w[j].w, o + 8 * j + 6);
                 }
+                tmem_st32(a0 + r.s * 32, o);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();                                        // (every lane has its words in registers, and A is written)
@@ -375,6 +351,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         const int q = warp & 3, half = (warp - EPI_WARP0) >> 2, row = q * 32 + lane;
         const uint32_t d0 = tmem + ((uint32_t)(q * 32) << 16) + half * 16, sb0 = sring_s + half * 64, sw0 = wsring_s + row * 4;
         Ring<RING> r;
+        Ring<NACC> acc;
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
             const Unit un = find_unit(p, u, kCols, tiles, ends);
@@ -386,29 +363,31 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             for (int a = 0; a < 4; a++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) C[a][j] = 0;
-            for (int g = 0; g < G; g++, shift ^= 16, r.next()) {
+            for (int g = 0; g < G; g++, shift ^= 16, r.next(), acc.next()) {
                 if (!(ok = wait_warp(done + r.s * 8, r.ph, ctl, 28))) break;
                 tc_fence_after();
-                const uint32_t slot = (r.s + RING * r.ph) * 512, sb = sb0 + slot, d = d0 + (r.s & 1) * kCols;
-                const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(lds32(sw0 + slot) >> shift))));
+                const uint32_t slot = (r.s + RING * r.ph) * 512, sb = sb0 + slot, d = d0 + acc.s * kCols;
+                const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(lds32(sw0 + slot) >> shift))) * 0.0625f);
                 const uint64_t s2 = pack2(s, s);
 #pragma unroll
                 for (int a = 0; a < 4; a++) {
                     if (a >= chunks) break;
-                    uint64_t f[8], v[8];
+                    uint64_t f[8];
+                    uint32_t v[16];
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
                         const uint4 b = lds128(sb + a * 128 + j * 8);
                         f[j] = mul2p(s2, pack2(b.x, b.y));
                         f[j + 1] = mul2p(s2, pack2(b.z, b.w));
                     }
-                    tmem_ld16_pairs(d + a * 32, v);
+                    tmem_ld16_now(d + a * 32, v);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) fma2p(C[a][j], v[j], f[j]);
+                    for (int j = 0; j < 8; j++)
+                        fma2p(C[a][j], pack2(__float_as_uint((float)(int)v[2 * j]), __float_as_uint((float)(int)v[2 * j + 1])), f[j]);
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_at(acc_free + (r.s & 1) * 8);
+                if (lane == 0) mbar_arrive_at(acc_free + acc.s * 8);
             }
             if (!ok) break;
             const float bias = p.bias ? p.bias[weight_row<GATED>(p, un, row)] : 0.f;
@@ -464,19 +443,19 @@ size_t smem_bytes(const Params& p) {
 }  // namespace
 
 int run_tiles(const char* kn, const LaunchCtx& c, const Params& p) {
-    const size_t bytes = (size_t)p.m * p.K * 2;
-    __half* xh = static_cast<__half*>(engine_scratch(bytes));
-    FM_REQUIRE(xh, kn, "the engine workspace cannot grow to %zu bytes here (inside a capture: raise FM_SCRATCH_MB)", bytes);
+    const size_t bytes = (size_t)p.m * p.K;
+    int8_t* xq = static_cast<int8_t*>(engine_scratch(bytes));
+    FM_REQUIRE(xq, kn, "the engine workspace cannot grow to %zu bytes here (inside a capture: raise FM_SCRATCH_MB)", bytes);
     CUtensorMap map_w;
     RowMaps map_x;
     const uint64_t wrows = (uint64_t)p.n_exp * p.N * (p.gated ? 2 : 1);
     bool ok = wrows < 0x7fffffff && encode_bytes_box_map(&map_w, p.wq, wrows, (uint64_t)p.K / 2, 64, 64);
-    for (int b = 0; b < 4; b++) ok = ok && encode_bytes_box_map(&map_x.box[b], xh, (uint64_t)p.m, (uint64_t)p.K * 2, 128, 128 >> b);
+    for (int b = 0; b < 4; b++) ok = ok && encode_bytes_box_map(&map_x.box[b], xq, (uint64_t)p.m, (uint64_t)p.K, 128, 128 >> b);
     FM_REQUIRE(ok, kn, "the tensor maps of %llu rows of weights and %d rows of x were refused (K=%d)", (unsigned long long)wrows, p.m, p.K);
-    const size_t n = (size_t)p.m * (p.K / 16);
+    const size_t n = (size_t)p.m * (p.K / 32);
     size_t eb = (n + 255) / 256;
     if (eb > (size_t)c.sm_count * 16) eb = (size_t)c.sm_count * 16;
-    cudaError_t e = launch_kernel(expand_codes_kernel, dim3((unsigned)eb), dim3(256), 0, c.stream, pdl_enabled(), p, xh);
+    cudaError_t e = launch_kernel(order_codes_kernel, dim3((unsigned)eb), dim3(256), 0, c.stream, pdl_enabled(), p, xq);
     if (e != cudaSuccess) return cuda_fail(kn, e);
     const int rc = after_launch(kn);
     if (rc != FM_OK) return rc;

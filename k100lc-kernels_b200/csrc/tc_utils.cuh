@@ -95,9 +95,9 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
                  :: "memory");
 }
 
-// kind::f16 with the A operand in tensor memory (two 16-bit values per column) and B in shared memory
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+// kind::i8 with the A operand in tensor memory (four values per column) and B in shared memory
+__device__ __forceinline__ void tc_mma_i8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n}"
                  ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
 // 32 lanes x 32 columns of 32-bit: thread t of the warp writes lane t, columns c..c+31 (complete after tmem_st_wait)
@@ -111,14 +111,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
                    "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 32 lanes x 16 columns, waited for: thread t gets columns c..c+15 of lane t as eight 64-bit pairs
-__device__ __forceinline__ void tmem_ld16_pairs(uint32_t taddr, uint64_t (&r)[8]) {
-    asm volatile("{\n.reg .b32 t<16>;\n"
-                 "tcgen05.ld.sync.aligned.32x32b.x16.b32 {t0,t1,t2,t3,t4,t5,t6,t7,t8,t9,t10,t11,t12,t13,t14,t15}, [%8];\n"
-                 "tcgen05.wait::ld.sync.aligned;\n"
-                 "mov.b64 %0, {t0,t1};\nmov.b64 %1, {t2,t3};\nmov.b64 %2, {t4,t5};\nmov.b64 %3, {t6,t7};\n"
-                 "mov.b64 %4, {t8,t9};\nmov.b64 %5, {t10,t11};\nmov.b64 %6, {t12,t13};\nmov.b64 %7, {t14,t15};\n}"
-                 : "=l"(r[0]), "=l"(r[1]), "=l"(r[2]), "=l"(r[3]), "=l"(r[4]), "=l"(r[5]), "=l"(r[6]), "=l"(r[7]) : "r"(taddr) : "memory");
+// 32 lanes x 16 columns, waited for: thread t gets columns c..c+15 of lane t
+__device__ __forceinline__ void tmem_ld16_now(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
 }
 // the barrier operations by 32-bit shared address: ring positions become one add
 __device__ __forceinline__ bool mbar_try_wait_at(uint32_t b, uint32_t parity) {
