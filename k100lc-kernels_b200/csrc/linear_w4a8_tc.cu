@@ -8,14 +8,14 @@
 // (kind::f16, whose fp32 accumulators need no conversion, was a third slower: its expansion takes nine instructions for
 // eight weights, its rows of x twice the bytes, and its MMAs leave tensor memory for two accumulators instead of three.)
 //
-// Roles of the 20 warps of the persistent CTA, joined by mbarriers (every wait is bounded):
+// Roles of the 16 warps of the persistent CTA, joined by mbarriers (every wait is bounded):
 //   * one warp copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring;
-//   * eight warps expand them: a thread owns a weight row, reads its 64 bytes and writes 128 to tensor memory, from where
+//   * four warps expand them: a thread owns a weight row, reads its 64 bytes and writes 128 to tensor memory, from where
 //     the MMA takes its A operand;
 //   * one warp copies the rows of x by TMA, put into bucket order and into the k order of the nibbles once per call by a
 //     small kernel in front; it also fetches the scales of the weight rows and of the rows of x (cp.async);
 //   * two warps issue the MMAs of the even and the odd groups, into three accumulators in turn;
-//   * eight warps drain the accumulators: C[m, n] = fmaf(float(I), ws * asc, C) in registers, then the epilogue.
+//   * eight warps, four for the even and four for the odd groups, drain the accumulators: C[m, n] = fmaf(float(I), ws * asc, C) in registers, then the epilogue.
 #include <cuda.h>
 
 #include "device_utils.cuh"
@@ -35,10 +35,10 @@ constexpr int BP = 8;                               // stages of packed weights
 constexpr int SLOTS = 8;                            // stages of scales (reuse distance: see where they are fetched)
 constexpr int kLag = 2;                             // steps between issuing a fetch of scales and publishing it
 constexpr int B_BYTES = kCols * 128, BP_BYTES = 128 * 64;
-constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 3, EXP_WARP0 = 4, EPI_WARP0 = 12, kThreads = 20 * 32;
-// 640 threads start with 96 registers each (61 440 of the file); the shares below add up to no more
-constexpr int kRegsIssue = 72, kRegsExpand = 72, kRegsEpilogue = 128;
-static_assert(kRegsIssue + 2 * kRegsExpand + 2 * kRegsEpilogue <= 480, "register shares of the five warpgroups");
+constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 3, EXP_WARP0 = 4, EPI_WARP0 = 8, kThreads = 16 * 32;
+// 512 threads start with 128 registers each; the shares below add up to no more
+constexpr int kRegsIssue = 72, kRegsExpand = 72, kRegsEpilogue = 184;
+static_assert(kRegsIssue + kRegsExpand + 2 * kRegsEpilogue <= 512, "register shares of the four warpgroups");
 static_assert(SLOTS >= RING + NACC, "a scale slot is rewritten RING steps ahead of the MMAs, which are NACC ahead of the epilogue");
 constexpr int kSpin = 1 << 17;
 constexpr uint32_t kTmemCols = 512, kTmemA = NACC * kCols;   // accumulators, then A: 4 x 32 columns
@@ -142,8 +142,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
     uint8_t* wring = bring + RING * B_BYTES;                         // BP x [128 rows][64 bytes]
     float* sring = reinterpret_cast<float*>(wring + BP * BP_BYTES);  // SLOTS x [128]
     uint32_t* wsring = reinterpret_cast<uint32_t*>(sring + SLOTS * kCols);   // SLOTS x [128]: the word that holds the weight row's scale
-    float* xch = reinterpret_cast<float*>(wsring + SLOTS * 128);     // [32 columns][128 rows] of sums on their way out
-    Control* ctl = reinterpret_cast<Control*>(xch + 32 * 128);
+    float* xch = reinterpret_cast<float*>(wsring + SLOTS * 128);     // 2 x [32 columns][128 rows] of partial sums on their way out
+    Control* ctl = reinterpret_cast<Control*>(xch + 2 * 32 * 128);
     int* ends = reinterpret_cast<int*>(ctl + 1);                     // [n_exp]
     __shared__ Buckets bk;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -160,7 +160,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             mbar_init(&ctl->b_full[i], 2);
             mbar_init(&ctl->done[i], 1);
         }
-        for (int i = 0; i < NACC; i++) mbar_init(&ctl->acc_free[i], 8);
+        for (int i = 0; i < NACC; i++) mbar_init(&ctl->acc_free[i], 4);
         for (int i = 0; i < 2; i++) mbar_init(&ctl->drain[i], 1);
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -305,21 +305,16 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         }
     } else if (warp < EPI_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsExpand));
-        // ==================================================================== expansion of the weights: even and odd steps
-        const uint32_t set = (warp - EXP_WARP0) >> 2, q = warp & 3, row = q * 32 + lane;
+        // ==================================================================== expansion of the weights
+        const uint32_t q = warp & 3, row = q * 32 + lane;
         const uint32_t a0 = tmem + ((uint32_t)(q * 32) << 16) + kTmemA;
         const uint32_t x = ((row >> 1) & 3) << 4;                    // 64-byte swizzle: chunk ^= (row / 2) % 4
         const uint32_t w0 = wring_s + row * 64 + x, w1 = wring_s + row * 64 + (16 ^ x), w2 = wring_s + row * 64 + (32 ^ x), w3 = wring_s + row * 64 + (48 ^ x);
         Ring<BP> rp;
         Ring<RING> r;
-        uint32_t parity = 0;
-        if (set) {
-            rp.next();
-            r.next();
-        }
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
-            for (int g = set ^ parity; g < G; g += 2, rp.next2(), r.next2()) {
+            for (int g = 0; g < G; g++, rp.next(), r.next()) {
                 if (!(ok = wait_warp(bp_full + rp.s * 8, rp.ph, ctl, 26))) break;
                 const uint32_t at = rp.s * BP_BYTES;
                 const uint4 w[4] = {lds128(w0 + at), lds128(w1 + at), lds128(w2 + at), lds128(w3 + at)};
@@ -342,45 +337,52 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                     mbar_arrive_at(a_full + r.s * 8);
                 }
             }
-            parity ^= G & 1;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
         // ==================================================================== epilogue
-        // warp: lanes 32 q .. of the accumulators, 16-column chunks half, half + 2, ... of the tile
-        const int q = warp & 3, half = (warp - EPI_WARP0) >> 2, row = q * 32 + lane;
-        const uint32_t d0 = tmem + ((uint32_t)(q * 32) << 16) + half * 16, sb0 = sring_s + half * 64, sw0 = wsring_s + row * 4;
+        // Two sets of four warps, one for the even and one for the odd steps, so that a set has two step times for its chain of
+        // waits, loads and sums; a tile's two partial sums meet on their way out.  warp: lanes 32 q .. of the accumulators
+        const uint32_t set = (warp - EPI_WARP0) >> 2, q = warp & 3, row = q * 32 + lane;
+        const uint32_t d0 = tmem + ((uint32_t)(q * 32) << 16), sw0 = wsring_s + row * 4;
+        float* plane = xch + set * (32 * 128);
         Ring<RING> r;
         Ring<NACC> acc;
-        bool ok = true;
-        for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+        uint32_t parity = 0;                                         // of the first step of the tile
+        if (set) {
+            r.next();
+            acc.next();
+        }
+        for (int u = blockIdx.x; u < total; u += gridDim.x) {
             const Unit un = find_unit(p, u, kCols, tiles, ends);
-            const int n0 = un.tile * ROWS, chunks = (un.count - half * 16 + 31) >> 5;
-            // which half of its word the scale of group g is: by g's parity
-            uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, row) * G) >> 1) << 4 & 16;
-            uint64_t C[4][8];                                        // pairs of neighbouring columns
+            const int n0 = un.tile * ROWS, chunks = (un.count + 15) >> 4;
+            // which half of its word the scale of a group is: by the group's parity, one for the set's groups of a tile
+            const uint32_t shift = ((uint32_t)(reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, row) * G) >> 1) ^ set ^ parity) << 4 & 16;
+            const float bias = p.bias && set == 0 ? p.bias[weight_row<GATED>(p, un, row)] : 0.f;
+            bool ok = true;
+            uint64_t C[8][8];                                        // pairs of neighbouring columns
 #pragma unroll
-            for (int a = 0; a < 4; a++)
+            for (int a = 0; a < 8; a++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) C[a][j] = 0;
-            for (int g = 0; g < G; g++, shift ^= 16, r.next(), acc.next()) {
+            for (int g = set ^ parity; g < G; g += 2, r.next2(), acc.next2()) {
                 if (!(ok = wait_warp(done + r.s * 8, r.ph, ctl, 28))) break;
                 tc_fence_after();
-                const uint32_t slot = (r.s + RING * r.ph) * 512, sb = sb0 + slot, d = d0 + acc.s * kCols;
+                const uint32_t slot = (r.s + RING * r.ph) * 512, sb = sring_s + slot, d = d0 + acc.s * kCols;
                 const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(lds32(sw0 + slot) >> shift))) * 0.0625f);
                 const uint64_t s2 = pack2(s, s);
 #pragma unroll
-                for (int a = 0; a < 4; a++) {
+                for (int a = 0; a < 8; a++) {
                     if (a >= chunks) break;
                     uint64_t f[8];
                     uint32_t v[16];
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
-                        const uint4 b = lds128(sb + a * 128 + j * 8);
+                        const uint4 b = lds128(sb + a * 64 + j * 8);
                         f[j] = mul2p(s2, pack2(b.x, b.y));
                         f[j + 1] = mul2p(s2, pack2(b.z, b.w));
                     }
-                    tmem_ld16_now(d + a * 32, v);
+                    tmem_ld16_now(d + a * 16, v);
 #pragma unroll
                     for (int j = 0; j < 8; j++)
                         fma2p(C[a][j], pack2(__float_as_uint((float)(int)v[2 * j]), __float_as_uint((float)(int)v[2 * j + 1])), f[j]);
@@ -389,45 +391,54 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 __syncwarp();
                 if (lane == 0) mbar_arrive_at(acc_free + acc.s * 8);
             }
-            if (!ok) break;
-            const float bias = p.bias ? p.bias[weight_row<GATED>(p, un, row)] : 0.f;
+            parity ^= G & 1;
             // 32 columns at a time through shared memory, so that the loop with the activation stays rolled: unrolled over
-            // the registers it was 60 KB of code, and fetching that took 1.7 times as long as the tile's products
+            // the registers it was 60 KB of code, and fetching that took 1.7 times as long as the tile's products.  (A set that
+            // gave up a wait takes part in the barriers all the same; the last one of the tile tells all.)
+            const int t = threadIdx.x - EPI_WARP0 * 32;
+            const long long end = (long long)un.first + un.count;
 #pragma unroll
             for (int a = 0; a < 4; a++) {
                 if (a * 32 >= un.count) break;
-                const long long m0 = (long long)un.first + a * 32, end = (long long)un.first + un.count;
+                const long long m0 = (long long)un.first + a * 32;
+                if (a) asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    xch[(half * 16 + 2 * j) * 128 + row] = __uint_as_float((uint32_t)C[a][j]) + bias;
-                    xch[(half * 16 + 2 * j + 1) * 128 + row] = __uint_as_float((uint32_t)(C[a][j] >> 32)) + bias;
+                for (int j = 0; j < 16; j++) {
+                    const uint64_t v = C[2 * a + (j >> 3)][j & 7];
+                    plane[2 * j * 128 + row] = __uint_as_float((uint32_t)v) + bias;
+                    plane[(2 * j + 1) * 128 + row] = __uint_as_float((uint32_t)(v >> 32)) + bias;
                 }
-                if (GATED) {                                         // gate lane r meets up lane 64 + r
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    const int t = threadIdx.x - EPI_WARP0 * 32, gr = t & 63;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (GATED) {                                         // gate lane gr meets up lane 64 + gr
+                    const int gr = t & 63;
                     if (n0 + gr < p.N)
 #pragma unroll 1
                         for (int col = t >> 6; col < 32 && m0 + col < end; col += 16) {
                             float v[4], up[4];
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                v[i] = xch[(col + 4 * i) * 128 + gr];
-                                up[i] = xch[(col + 4 * i) * 128 + 64 + gr];
+                                const float* at = xch + (col + 4 * i) * 128 + gr;
+                                v[i] = at[0] + at[32 * 128];
+                                up[i] = at[64] + at[32 * 128 + 64];
                             }
                             finish<4, true>(p, m0 + col, 4, end, n0 + gr, v, up);
                         }
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                } else if (n0 + row < p.N) {                         // a thread reads what it wrote
+                } else if (n0 + (int)row < p.N) {
 #pragma unroll 1
-                    for (int col = half * 16; col < half * 16 + 16 && m0 + col < end; col += 4) {
+                    for (int col = set * 16; col < (int)set * 16 + 16 && m0 + col < end; col += 4) {
                         float v[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) v[i] = xch[(col + i) * 128 + row];
+                        for (int i = 0; i < 4; i++) {
+                            const float* at = xch + (col + i) * 128 + row;
+                            v[i] = at[0] + at[32 * 128];
+                        }
                         finish<4, false>(p, m0 + col, 1, end, n0 + row, v, v);
                     }
                 }
             }
-            __syncwarp();
+            int all;
+            asm volatile("{\n.reg .pred p, q;\nsetp.ne.s32 p, %1, 0;\nbar.red.and.pred q, 1, 256, p;\nselp.s32 %0, 1, 0, q;\n}" : "=r"(all) : "r"((int)ok) : "memory");
+            if (!all) break;
         }
     }
     tc_fence_before();
@@ -437,7 +448,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 }
 
 size_t smem_bytes(const Params& p) {
-    return 1024 + RING * B_BYTES + BP * BP_BYTES + SLOTS * (kCols + 128) * 4 + 32 * 128 * 4 + sizeof(Control) + (size_t)p.n_exp * 4;
+    return 1024 + RING * B_BYTES + BP * BP_BYTES + SLOTS * (kCols + 128) * 4 + 2 * 32 * 128 * 4 + sizeof(Control) + (size_t)p.n_exp * 4;
 }
 
 }  // namespace
