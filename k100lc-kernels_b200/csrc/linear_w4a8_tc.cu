@@ -5,8 +5,9 @@
 // lanes of an accumulator, up to 128 rows of a bucket its columns, so that a short bucket costs a narrow MMA and not a
 // padded tile.  tcgen05.mma.kind::i8 forms the exact integer of a 128-group; the weights enter as 16 w, a nibble in the
 // upper half of its byte, which takes two logic instructions for eight of them, and the 16 is divided out of their scale.
-// (kind::f16, whose fp32 accumulators need no conversion, was a third slower: its expansion takes nine instructions for
-// eight weights, its rows of x twice the bytes, and its MMAs leave tensor memory for two accumulators instead of three.)
+// (kind::f16, whose fp32 accumulators need no conversion, took 526 us where this took 480 for 2048 x 17408 x 5120: its
+// expansion takes nine instructions for eight weights, its rows of x twice the bytes, and its A operand leaves tensor memory
+// for two accumulators instead of three.)
 //
 // Roles of the 16 warps of the persistent CTA, joined by mbarriers (every wait is bounded):
 //   * one warp copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring;
@@ -15,7 +16,8 @@
 //   * one warp copies the rows of x by TMA, put into bucket order and into the k order of the nibbles once per call by a
 //     small kernel in front; it also fetches the scales of the weight rows and of the rows of x (cp.async);
 //   * two warps issue the MMAs of the even and the odd groups, into three accumulators in turn;
-//   * eight warps, four for the even and four for the odd groups, drain the accumulators: C[m, n] = fmaf(float(I), ws * asc, C) in registers, then the epilogue.
+//   * eight warps, four for the even and four for the odd groups, drain the accumulators: C[m, n] = fmaf(float(I), ws * asc,
+//     C) in registers, then the epilogue.
 #include <cuda.h>
 
 #include "device_utils.cuh"
@@ -47,7 +49,7 @@ static_assert(NACC * kCols + RING * 32 <= 512, "tensor memory");
 struct __align__(16) Control {
     uint64_t bp_full[BP], bp_free[BP];
     uint64_t a_full[RING], b_full[RING], done[RING];
-    uint64_t acc_free[NACC], drain[2];
+    uint64_t acc_full[NACC], acc_free[NACC], drain[2];
     uint32_t tmem_base;
     volatile int abort;
 };
@@ -114,6 +116,12 @@ __device__ __forceinline__ size_t weight_row(const Params& p, const Unit& u, int
     return (size_t)u.expert * 2 * p.N + (row < 64 ? 0 : p.N) + min(u.tile * 64 + (row & 63), p.N - 1);
 }
 
+// A wait names a phase by its parity, so a waiter must never be two phases behind its barrier.  The copy and expansion roles
+// wait for the step that frees the stage they are about to fill, which cannot be used again before they have filled it; the
+// MMAs wait for what is filled only once they have used it; a set of the epilogue waits on the barrier of an accumulator,
+// which is not given back before the set has drained it.  (The sets are not in step with each other: on the barriers of the
+// stages one of them could fall two phases behind.)
+//
 // Position in a ring of N stages and the parity of its phase there.  A wait for the other parity passes at once in the first
 // round: the phase before a barrier's first counts as complete.
 template <int N>
@@ -160,7 +168,10 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             mbar_init(&ctl->b_full[i], 2);
             mbar_init(&ctl->done[i], 1);
         }
-        for (int i = 0; i < NACC; i++) mbar_init(&ctl->acc_free[i], 4);
+        for (int i = 0; i < NACC; i++) {
+            mbar_init(&ctl->acc_full[i], 1);
+            mbar_init(&ctl->acc_free[i], 4);
+        }
         for (int i = 0; i < 2; i++) mbar_init(&ctl->drain[i], 1);
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -175,7 +186,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 
     const uint32_t bring_s = smem_u32(bring), wring_s = smem_u32(wring), sring_s = smem_u32(sring), wsring_s = smem_u32(wsring);
     const uint32_t bp_full = smem_u32(ctl->bp_full), bp_free = smem_u32(ctl->bp_free), a_full = smem_u32(ctl->a_full), b_full = smem_u32(ctl->b_full);
-    const uint32_t done = smem_u32(ctl->done), acc_free = smem_u32(ctl->acc_free);
+    const uint32_t done = smem_u32(ctl->done), acc_full = smem_u32(ctl->acc_full), acc_free = smem_u32(ctl->acc_free);
     if (warp < EXP_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         // In these roles the whole warp walks the steps and one lane is elected to issue: a single lane that waits alone polls
@@ -292,6 +303,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 #pragma unroll
                         for (int j = 0; j < 4; j++)                  // 32 k each: 8 columns of A, 32 bytes of B
                             tc_mma_i8_ts(d, a + j * 8, bd + j * 2, idesc, j > 0);
+                        tc_commit_at(acc_full + acc.s * 8);
                         tc_commit_at(done + r.s * 8);
                     }
                     __syncwarp();
@@ -366,7 +378,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 #pragma unroll
                 for (int j = 0; j < 8; j++) C[a][j] = 0;
             for (int g = set ^ parity; g < G; g += 2, r.next2(), acc.next2()) {
-                if (!(ok = wait_warp(done + r.s * 8, r.ph, ctl, 28))) break;
+                if (!(ok = wait_warp(acc_full + acc.s * 8, acc.ph, ctl, 28))) break;
                 tc_fence_after();
                 const uint32_t slot = (r.s + RING * r.ph) * 512, sb = sring_s + slot, d = d0 + acc.s * kCols;
                 const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(lds32(sw0 + slot) >> shift))) * 0.0625f);
