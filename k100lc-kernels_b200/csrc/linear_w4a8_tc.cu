@@ -10,11 +10,12 @@
 // for two accumulators instead of three.)
 //
 // Roles of the 16 warps of the persistent CTA, joined by mbarriers (every wait is bounded):
-//   * one warp copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring;
+//   * one warp copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring, and the scales of the weight rows
+//     and of the rows of x (cp.async);
 //   * four warps expand them: a thread owns a weight row, reads its 64 bytes and writes 128 to tensor memory, from where
 //     the MMA takes its A operand;
 //   * one warp copies the rows of x by TMA, put into bucket order and into the k order of the nibbles once per call by a
-//     small kernel in front; it also fetches the scales of the weight rows and of the rows of x (cp.async);
+//     small kernel in front;
 //   * two warps issue the MMAs of the even and the odd groups, into three accumulators in turn;
 //   * eight warps, four for the even and four for the odd groups, drain the accumulators: C[m, n] = fmaf(float(I), ws * asc,
 //     C) in registers, then the epilogue.
@@ -34,20 +35,20 @@ constexpr int kCols = 128;                          // rows of x per tile
 constexpr int RING = 4;                             // stages of A (tensor memory), B (shared memory) and "step done" barriers
 constexpr int NACC = 3;                             // accumulators
 constexpr int BP = 8;                               // stages of packed weights
-constexpr int SLOTS = 8;                            // stages of scales (reuse distance: see where they are fetched)
-constexpr int kLag = 2;                             // steps between issuing a fetch of scales and publishing it
+constexpr int SLOTS = 16;                           // stages of scales (reuse distance: see where they are fetched)
+constexpr int kLag = 6;                             // steps between issuing a fetch of scales and publishing it
 constexpr int B_BYTES = kCols * 128, BP_BYTES = 128 * 64;
 constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 3, EXP_WARP0 = 4, EPI_WARP0 = 8, kThreads = 16 * 32;
 // 512 threads start with 128 registers each; the shares below add up to no more
 constexpr int kRegsIssue = 72, kRegsExpand = 72, kRegsEpilogue = 184;
 static_assert(kRegsIssue + kRegsExpand + 2 * kRegsEpilogue <= 512, "register shares of the four warpgroups");
-static_assert(SLOTS >= RING + NACC, "a scale slot is rewritten RING steps ahead of the MMAs, which are NACC ahead of the epilogue");
+static_assert(SLOTS >= BP + RING + NACC && kLag < BP, "see where the scales are fetched");
 constexpr int kSpin = 1 << 17;
 constexpr uint32_t kTmemCols = 512, kTmemA = NACC * kCols;   // accumulators, then A: 4 x 32 columns
 static_assert(NACC * kCols + RING * 32 <= 512, "tensor memory");
 
 struct __align__(16) Control {
-    uint64_t bp_full[BP], bp_free[BP];
+    uint64_t bp_full[BP], bp_free[BP], s_full[SLOTS];
     uint64_t a_full[RING], b_full[RING], done[RING];
     uint64_t acc_full[NACC], acc_free[NACC], drain[2];
     uint32_t tmem_base;
@@ -119,7 +120,7 @@ __device__ __forceinline__ size_t weight_row(const Params& p, const Unit& u, int
 // A wait names a phase by its parity, so a waiter must never be two phases behind its barrier.  The copy and expansion roles
 // wait for the step that frees the stage they are about to fill, which cannot be used again before they have filled it; the
 // MMAs wait for what is filled only once they have used it; a set of the epilogue waits on the barrier of an accumulator,
-// which is not given back before the set has drained it.  (The sets are not in step with each other: on the barriers of the
+// which is not given back before the set has drained it, and on those of the scales (see there).  (The sets are not in step with each other: on the barriers of the
 // stages one of them could fall two phases behind.)
 //
 // Position in a ring of N stages and the parity of its phase there.  A wait for the other parity passes at once in the first
@@ -136,7 +137,6 @@ struct Ring {
         ph ^= s < 2 ? 1u : 0u;
     }
 };
-static_assert(SLOTS == 2 * RING, "a ring position and its phase name a slot");
 
 struct RowMaps { CUtensorMap box[4]; };             // boxes of 128, 64, 32 and 16 rows of x (a group)
 
@@ -165,13 +165,14 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         }
         for (int i = 0; i < RING; i++) {
             mbar_init(&ctl->a_full[i], 4);
-            mbar_init(&ctl->b_full[i], 2);
+            mbar_init(&ctl->b_full[i], 1);
             mbar_init(&ctl->done[i], 1);
         }
         for (int i = 0; i < NACC; i++) {
             mbar_init(&ctl->acc_full[i], 1);
             mbar_init(&ctl->acc_free[i], 4);
         }
+        for (int i = 0; i < SLOTS; i++) mbar_init(&ctl->s_full[i], 1);
         for (int i = 0; i < 2; i++) mbar_init(&ctl->drain[i], 1);
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -186,47 +187,25 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 
     const uint32_t bring_s = smem_u32(bring), wring_s = smem_u32(wring), sring_s = smem_u32(sring), wsring_s = smem_u32(wsring);
     const uint32_t bp_full = smem_u32(ctl->bp_full), bp_free = smem_u32(ctl->bp_free), a_full = smem_u32(ctl->a_full), b_full = smem_u32(ctl->b_full);
-    const uint32_t done = smem_u32(ctl->done), acc_full = smem_u32(ctl->acc_full), acc_free = smem_u32(ctl->acc_free);
+    const uint32_t s_full = smem_u32(ctl->s_full), done = smem_u32(ctl->done), acc_full = smem_u32(ctl->acc_full), acc_free = smem_u32(ctl->acc_free);
     if (warp < EXP_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         // In these roles the whole warp walks the steps and one lane is elected to issue: a single lane that waits alone polls
         // its barrier dozens of times a step, and descriptors stay in uniform registers.
         if (warp == WEIGHT_WARP) {
-            // ================================================================ packed weights
+            // ================================================================ packed weights and all scales
+            // A lane fetches the scales of four rows of x and the aligned words around those of four weight rows (a copy has at
+            // least four bytes; allocations are whole words).  They are published kLag steps later, when they have landed: two
+            // steps were less than the memory's latency and held the MMAs up.  Step it - BP has been expanded when its weights
+            // are overwritten, so the MMAs up to it - BP - RING have run, which were issued after the accumulators up to step
+            // it - BP - RING - NACC had been drained: nobody reads slot or barrier it % SLOTS any more.
             Ring<BP> r;
+            Ring<SLOTS> fetch, behind;
             int it = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const int y0 = un.expert * (GATED ? 2 * p.N : p.N) + un.tile * ROWS, y1 = y0 + (GATED ? p.N : 64);
-                for (int g = 0; g < G; g++, it++, r.next()) {
-                    if (!(ok = wait_warp(bp_free + r.s * 8, r.ph ^ 1, ctl, 21))) break;
-                    if (elect_one()) {
-                        const uint32_t bar = bp_full + r.s * 8, dst = wring_s + r.s * BP_BYTES;
-                        mbar_expect_tx_at(bar, BP_BYTES);
-                        tma_2d_at(dst, &map_w, g * 64, y0, bar);
-                        tma_2d_at(dst + BP_BYTES / 2, &map_w, g * 64, y1, bar);
-                    }
-                    __syncwarp();
-                }
-            }
-            if (ctl->abort)                                          // copies in flight land before the memory is given up
-                for (int j = it > BP ? it - BP : 0; j < it; j++)
-                    for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->bp_full[j % BP], (j / BP) & 1); i++) {}
-        } else if (warp == ROW_WARP) {
-            // ================================================================ rows of x and all scales
-            // A count of rows is a sum of boxes of 128, 64, 32 and 16: a box costs its issue, about 100 clocks, whatever it holds
-            // (16-row boxes throughout, 16 instructions a step, bound the tile at 1800 clocks; four-row gathers at 6000).
-            // A lane fetches the scales of four rows of x and the aligned words around those of four weight rows (a copy has at
-            // least four bytes; allocations are whole words).  Slot it % SLOTS was last read by the epilogue of step it - SLOTS:
-            // stage it % RING is free when the MMAs of step it - RING have run, which were issued after the accumulator of step
-            // it - RING - NACC had been drained.
-            Ring<RING> r, behind;
-            int it = 0;
-            bool ok = true;
-            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
-                const Unit un = find_unit(p, u, kCols, tiles, ends);
-                const int n16 = (un.count + 15) & ~15;
                 const float* sc[4];
                 uintptr_t wsc[4];
                 bool has[4];
@@ -237,6 +216,49 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                     sc[i] = p.asc + (sr < 0 ? 0 : (size_t)sr * G);
                     wsc[i] = reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, lane + 32 * i) * G);
                 }
+                for (int g = 0; g < G; g++, it++, r.next(), fetch.next()) {
+                    if (!(ok = wait_warp(bp_free + r.s * 8, r.ph ^ 1, ctl, 21))) break;
+                    if (elect_one()) {
+                        const uint32_t bar = bp_full + r.s * 8, dst = wring_s + r.s * BP_BYTES;
+                        mbar_expect_tx_at(bar, BP_BYTES);
+                        tma_2d_at(dst, &map_w, g * 64, y0, bar);
+                        tma_2d_at(dst + BP_BYTES / 2, &map_w, g * 64, y1, bar);
+                    }
+                    __syncwarp();
+                    const uint32_t slot = fetch.s * 512 + lane * 4;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        cp_async4(sring_s + slot + 128 * i, sc[i], has[i]);
+                        cp_async4(wsring_s + slot + 128 * i, reinterpret_cast<const void*>(wsc[i] & ~(uintptr_t)3), true);
+                        sc[i]++;
+                        wsc[i] += 2;
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (it >= kLag) {
+                        cp_async_wait<kLag>();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_at(s_full + behind.s * 8);
+                        behind.next();
+                    }
+                }
+            }
+            cp_async_wait<0>();
+            __syncwarp();
+            if (ok && lane == 0)
+                for (int j = it > kLag ? it - kLag : 0; j < it; j++, behind.next()) mbar_arrive_at(s_full + behind.s * 8);
+            if (ctl->abort)                                          // copies in flight land before the memory is given up
+                for (int j = it > BP ? it - BP : 0; j < it; j++)
+                    for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->bp_full[j % BP], (j / BP) & 1); i++) {}
+        } else if (warp == ROW_WARP) {
+            // ================================================================ rows of x
+            // A count of rows is a sum of boxes of 128, 64, 32 and 16: a box costs its issue, about 100 clocks, whatever it holds
+            // (16-row boxes throughout, 16 instructions a step, bound the tile at 1800 clocks; four-row gathers at 6000).
+            Ring<RING> r;
+            int it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+                const Unit un = find_unit(p, u, kCols, tiles, ends);
+                const int n16 = (un.count + 15) & ~15;
                 for (int g = 0; g < G; g++, it++, r.next()) {
                     if (!(ok = wait_warp(done + r.s * 8, r.ph ^ 1, ctl, 25))) break;
                     if (elect_one()) {
@@ -253,27 +275,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                             }
                     }
                     __syncwarp();
-                    const uint32_t slot = (r.s + RING * r.ph) * 512 + lane * 4;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        cp_async4(sring_s + slot + 128 * i, sc[i], has[i]);
-                        cp_async4(wsring_s + slot + 128 * i, reinterpret_cast<const void*>(wsc[i] & ~(uintptr_t)3), true);
-                        sc[i]++;
-                        wsc[i] += 2;
-                    }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    if (it >= kLag) {
-                        cp_async_wait<kLag>();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_at(b_full + behind.s * 8);
-                        behind.next();
-                    }
                 }
             }
-            cp_async_wait<0>();
-            __syncwarp();
-            if (ok && lane == 0)
-                for (int j = it > kLag ? it - kLag : 0; j < it; j++, behind.next()) mbar_arrive_at(b_full + behind.s * 8);
             if (ctl->abort)
                 for (int j = it > RING ? it - RING : 0; j < it; j++)
                     for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->b_full[j % RING], (j / RING) & 1); i++) {}
@@ -358,7 +361,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         const uint32_t set = (warp - EPI_WARP0) >> 2, q = warp & 3, row = q * 32 + lane;
         const uint32_t d0 = tmem + ((uint32_t)(q * 32) << 16), sw0 = wsring_s + row * 4;
         float* plane = xch + set * (32 * 128);
-        Ring<RING> r;
+        Ring<SLOTS> r;
         Ring<NACC> acc;
         uint32_t parity = 0;                                         // of the first step of the tile
         if (set) {
@@ -378,9 +381,10 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 #pragma unroll
                 for (int j = 0; j < 8; j++) C[a][j] = 0;
             for (int g = set ^ parity; g < G; g += 2, r.next2(), acc.next2()) {
+                if (!(ok = wait_warp(s_full + r.s * 8, r.ph, ctl, 29))) break;
                 if (!(ok = wait_warp(acc_full + acc.s * 8, acc.ph, ctl, 28))) break;
                 tc_fence_after();
-                const uint32_t slot = (r.s + RING * r.ph) * 512, sb = sring_s + slot, d = d0 + acc.s * kCols;
+                const uint32_t slot = r.s * 512, sb = sring_s + slot, d = d0 + acc.s * kCols;
                 const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(lds32(sw0 + slot) >> shift))) * 0.0625f);
                 const uint64_t s2 = pack2(s, s);
 #pragma unroll
