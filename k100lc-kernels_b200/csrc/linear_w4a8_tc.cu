@@ -50,7 +50,7 @@ static_assert(NACC * kCols + RING * 32 <= 512, "tensor memory");
 struct __align__(16) Control {
     uint64_t bp_full[BP], bp_free[BP], s_full[SLOTS];
     uint64_t a_full[RING], b_full[RING], done[RING];
-    uint64_t acc_full[NACC], acc_free[NACC], drain[2];
+    uint64_t acc_full[2 * NACC], acc_free[2 * NACC], drain[2];
     uint32_t tmem_base;
     volatile int abort;
 };
@@ -117,11 +117,11 @@ __device__ __forceinline__ size_t weight_row(const Params& p, const Unit& u, int
     return (size_t)u.expert * 2 * p.N + (row < 64 ? 0 : p.N) + min(u.tile * 64 + (row & 63), p.N - 1);
 }
 
-// A wait names a phase by its parity, so a waiter must never be two phases behind its barrier.  The copy and expansion roles
-// wait for the step that frees the stage they are about to fill, which cannot be used again before they have filled it; the
-// MMAs wait for what is filled only once they have used it; a set of the epilogue waits on the barrier of an accumulator,
-// which is not given back before the set has drained it, and on those of the scales (see there).  (The sets are not in step with each other: on the barriers of the
-// stages one of them could fall two phases behind.)
+// A wait names a phase by its parity, so a waiter must see every phase of its barrier: one phase late or early, the parity is
+// the same and the wait passes at once.  The copy and expansion roles wait for the step that frees the stage they are about to
+// fill, step by step.  The issuers and the sets of the epilogue take every other step: of the stages, an even number, each has
+// its own; the three accumulators change hands, so each has two pairs of barriers, for the even and the odd steps: step it
+// fills acc_full[it % 6], is drained by acc_free[it % 6] and takes over from step it - 3.
 //
 // Position in a ring of N stages and the parity of its phase there.  A wait for the other parity passes at once in the first
 // round: the phase before a barrier's first counts as complete.
@@ -168,7 +168,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             mbar_init(&ctl->b_full[i], 1);
             mbar_init(&ctl->done[i], 1);
         }
-        for (int i = 0; i < NACC; i++) {
+        for (int i = 0; i < 2 * NACC; i++) {
             mbar_init(&ctl->acc_full[i], 1);
             mbar_init(&ctl->acc_free[i], 4);
         }
@@ -285,7 +285,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             const uint32_t par = warp - MMA_WARP;
             const uint64_t bdesc0 = smem_desc_sw128(bring_s);
             Ring<RING> r;
-            Ring<NACC> acc;
+            Ring<2 * NACC> acc;
             uint32_t parity = 0;                                     // of the first step of the tile
             if (par) {
                 r.next();
@@ -298,10 +298,11 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 for (int g = par ^ parity; g < G; g += 2, r.next2(), acc.next2()) {
                     if (!(ok = wait_warp(a_full + r.s * 8, r.ph, ctl, 23))) break;
                     if (!(ok = wait_warp(b_full + r.s * 8, r.ph, ctl, 24))) break;
-                    if (!(ok = wait_warp(acc_free + acc.s * 8, acc.ph ^ 1, ctl, 22))) break;
+                    const uint32_t late = acc.s >= NACC, d_at = late ? acc.s - NACC : acc.s;
+                    if (!(ok = wait_warp(acc_free + (late ? d_at : d_at + NACC) * 8, acc.ph ^ 1 ^ late, ctl, 22))) break;
                     tc_fence_after();
                     const uint64_t bd = bdesc0 + (uint64_t)(r.s * (B_BYTES >> 4));
-                    const uint32_t d = tmem + acc.s * kCols, a = tmem + kTmemA + r.s * 32;
+                    const uint32_t d = tmem + d_at * kCols, a = tmem + kTmemA + r.s * 32;
                     if (elect_one()) {
 #pragma unroll
                         for (int j = 0; j < 4; j++)                  // 32 k each: 8 columns of A, 32 bytes of B
@@ -362,7 +363,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         const uint32_t d0 = tmem + ((uint32_t)(q * 32) << 16), sw0 = wsring_s + row * 4;
         float* plane = xch + set * (32 * 128);
         Ring<SLOTS> r;
-        Ring<NACC> acc;
+        Ring<2 * NACC> acc;
         uint32_t parity = 0;                                         // of the first step of the tile
         if (set) {
             r.next();
@@ -384,7 +385,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 if (!(ok = wait_warp(s_full + r.s * 8, r.ph, ctl, 29))) break;
                 if (!(ok = wait_warp(acc_full + acc.s * 8, acc.ph, ctl, 28))) break;
                 tc_fence_after();
-                const uint32_t slot = r.s * 512, sb = sring_s + slot, d = d0 + acc.s * kCols;
+                const uint32_t slot = r.s * 512, sb = sring_s + slot, d = d0 + (acc.s >= NACC ? acc.s - NACC : acc.s) * kCols;
                 const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(lds32(sw0 + slot) >> shift))) * 0.0625f);
                 const uint64_t s2 = pack2(s, s);
 #pragma unroll
