@@ -150,8 +150,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
     uint8_t* wring = bring + RING * B_BYTES;                         // BP x [128 rows][64 bytes]
     float* sring = reinterpret_cast<float*>(wring + BP * BP_BYTES);  // SLOTS x [128]
     uint32_t* wsring = reinterpret_cast<uint32_t*>(sring + SLOTS * kCols);   // SLOTS x [128]: the word that holds the weight row's scale
-    float* xch = reinterpret_cast<float*>(wsring + SLOTS * 128);     // 2 x [32 columns][128 rows] of partial sums on their way out
-    Control* ctl = reinterpret_cast<Control*>(xch + 2 * 32 * 128);
+    float* xch = reinterpret_cast<float*>(wsring + SLOTS * 128);     // a set's [64 columns][128 rows] of sums on their way out, twice
+    Control* ctl = reinterpret_cast<Control*>(xch + 128 * 128);
     int* ends = reinterpret_cast<int*>(ctl + 1);                     // [n_exp]
     __shared__ Buckets bk;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -285,17 +285,20 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             const uint32_t par = warp - MMA_WARP;
             const uint64_t bdesc0 = smem_desc_sw128(bring_s);
             Ring<RING> r;
+            Ring<SLOTS> sc;
             Ring<2 * NACC> acc;
             uint32_t parity = 0;                                     // of the first step of the tile
             if (par) {
                 r.next();
+                sc.next();
                 acc.next();
             }
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const uint32_t idesc = instr_desc((un.count + 15) & ~15);
-                for (int g = par ^ parity; g < G; g += 2, r.next2(), acc.next2()) {
+                for (int g = par ^ parity; g < G; g += 2, r.next2(), sc.next2(), acc.next2()) {
+                    if (!(ok = wait_warp(s_full + sc.s * 8, sc.ph, ctl, 29))) break;     // (for the epilogue)
                     if (!(ok = wait_warp(a_full + r.s * 8, r.ph, ctl, 23))) break;
                     if (!(ok = wait_warp(b_full + r.s * 8, r.ph, ctl, 24))) break;
                     const uint32_t late = acc.s >= NACC, d_at = late ? acc.s - NACC : acc.s;
@@ -361,7 +364,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         // waits, loads and sums; a tile's two partial sums meet on their way out.  warp: lanes 32 q .. of the accumulators
         const uint32_t set = (warp - EPI_WARP0) >> 2, q = warp & 3, row = q * 32 + lane;
         const uint32_t d0 = tmem + ((uint32_t)(q * 32) << 16), sw0 = wsring_s + row * 4;
-        float* plane = xch + set * (32 * 128);
+        float *const mine = xch + set * (64 * 128), *const theirs = xch + (set ^ 1) * (64 * 128);
         Ring<SLOTS> r;
         Ring<2 * NACC> acc;
         uint32_t parity = 0;                                         // of the first step of the tile
@@ -374,7 +377,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             const int n0 = un.tile * ROWS, chunks = (un.count + 15) >> 4;
             // which half of its word the scale of a group is: by the group's parity, one for the set's groups of a tile
             const uint32_t shift = ((uint32_t)(reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, row) * G) >> 1) ^ set ^ parity) << 4 & 16;
-            const float bias = p.bias && set == 0 ? p.bias[weight_row<GATED>(p, un, row)] : 0.f;
+            const float bias = p.bias ? p.bias[weight_row<GATED>(p, un, row)] : 0.f;
             bool ok = true;
             uint64_t C[8][8];                                        // pairs of neighbouring columns
 #pragma unroll
@@ -382,7 +385,6 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 #pragma unroll
                 for (int j = 0; j < 8; j++) C[a][j] = 0;
             for (int g = set ^ parity; g < G; g += 2, r.next2(), acc.next2()) {
-                if (!(ok = wait_warp(s_full + r.s * 8, r.ph, ctl, 29))) break;
                 if (!(ok = wait_warp(acc_full + acc.s * 8, acc.ph, ctl, 28))) break;
                 tc_fence_after();
                 const uint32_t slot = r.s * 512, sb = sring_s + slot, d = d0 + (acc.s >= NACC ? acc.s - NACC : acc.s) * kCols;
@@ -409,50 +411,51 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 if (lane == 0) mbar_arrive_at(acc_free + acc.s * 8);
             }
             parity ^= G & 1;
-            // 32 columns at a time through shared memory, so that the loop with the activation stays rolled: unrolled over
-            // the registers it was 60 KB of code, and fetching that took 1.7 times as long as the tile's products.  (A set that
-            // gave up a wait takes part in the barriers all the same; the last one of the tile tells all.)
-            const int t = threadIdx.x - EPI_WARP0 * 32;
+            // The sets swap half of their partial sums through shared memory, set k keeping the 16-column pieces a with a % 2 ==
+            // k, and put the sums of those there as well, so that the loop with the activation is rolled and there once: code that
+            // runs once a tile is fetched once a tile.  (Unrolled over the registers it was 60 KB, and fetching that took 1.7
+            // times as long as the tile's products; four loops of 32 columns took 15000 clocks of 57000.)  A warp that gave up a
+            // wait takes part in the barriers all the same; the last one of the tile tells all.
+            const int t = threadIdx.x & 127;
             const long long end = (long long)un.first + un.count;
 #pragma unroll
-            for (int a = 0; a < 4; a++) {
-                if (a * 32 >= un.count) break;
-                const long long m0 = (long long)un.first + a * 32;
-                if (a) asm volatile("bar.sync 1, 256;" ::: "memory");
+            for (int a = 0; a < 8; a += 2) {                         // (by static index: C stays in registers)
+                if (a >= chunks) break;
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const uint64_t v = C[2 * a + (j >> 3)][j & 7];
-                    plane[2 * j * 128 + row] = __uint_as_float((uint32_t)v) + bias;
-                    plane[(2 * j + 1) * 128 + row] = __uint_as_float((uint32_t)(v >> 32)) + bias;
-                }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (GATED) {                                         // gate lane gr meets up lane 64 + gr
-                    const int gr = t & 63;
-                    if (n0 + gr < p.N)
-#pragma unroll 1
-                        for (int col = t >> 6; col < 32 && m0 + col < end; col += 16) {
-                            float v[4], up[4];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const float* at = xch + (col + 4 * i) * 128 + gr;
-                                v[i] = at[0] + at[32 * 128];
-                                up[i] = at[64] + at[32 * 128 + 64];
-                            }
-                            finish<4, true>(p, m0 + col, 4, end, n0 + gr, v, up);
-                        }
-                } else if (n0 + (int)row < p.N) {
-#pragma unroll 1
-                    for (int col = set * 16; col < (int)set * 16 + 16 && m0 + col < end; col += 4) {
-                        float v[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float* at = xch + (col + i) * 128 + row;
-                            v[i] = at[0] + at[32 * 128];
-                        }
-                        finish<4, false>(p, m0 + col, 1, end, n0 + row, v, v);
-                    }
+                for (int j = 0; j < 8; j++) {
+                    const uint64_t c = set ? C[a][j] : C[a + 1][j];
+                    theirs[(a * 8 + 2 * j) * 128 + row] = __uint_as_float((uint32_t)c);
+                    theirs[(a * 8 + 2 * j + 1) * 128 + row] = __uint_as_float((uint32_t)(c >> 32));
                 }
             }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll
+            for (int a = 0; a < 8; a += 2) {
+                if (a >= chunks) break;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint64_t c = set ? C[a + 1][j] : C[a][j];
+                    float* at = mine + (a * 8 + 2 * j) * 128 + row;
+                    at[0] += __uint_as_float((uint32_t)c) + bias;
+                    at[128] += __uint_as_float((uint32_t)(c >> 32)) + bias;
+                }
+            }
+            if (GATED) asm volatile("bar.sync %0, 128;" ::"r"(2 + set) : "memory");          // gate lane gr meets up lane 64 + gr
+            const int n = n0 + (GATED ? t & 63 : (int)row);
+            if (n < p.N)
+#pragma unroll 1
+                for (int i = GATED ? t >> 6 << 2 : 0; i < 64; i += GATED ? 8 : 4) {
+                    const long long m = (long long)un.first + ((i & 48) * 2 + set * 16 + (i & 15));
+                    if (m >= end) break;
+                    const float* at = mine + i * 128 + n - n0;
+                    float v[4], up[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        v[k] = at[k * 128];
+                        up[k] = GATED ? at[k * 128 + 64] : 0.f;
+                    }
+                    finish<4, GATED>(p, m, 1, end, n, v, up);
+                }
             int all;
             asm volatile("{\n.reg .pred p, q;\nsetp.ne.s32 p, %1, 0;\nbar.red.and.pred q, 1, 256, p;\nselp.s32 %0, 1, 0, q;\n}" : "=r"(all) : "r"((int)ok) : "memory");
             if (!all) break;
@@ -465,7 +468,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 }
 
 size_t smem_bytes(const Params& p) {
-    return 1024 + RING * B_BYTES + BP * BP_BYTES + SLOTS * (kCols + 128) * 4 + 2 * 32 * 128 * 4 + sizeof(Control) + (size_t)p.n_exp * 4;
+    return 1024 + RING * B_BYTES + BP * BP_BYTES + SLOTS * (kCols + 128) * 4 + 128 * 128 * 4 + sizeof(Control) + (size_t)p.n_exp * 4;
 }
 
 }  // namespace
