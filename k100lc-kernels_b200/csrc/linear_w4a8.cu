@@ -54,6 +54,23 @@ __device__ __forceinline__ uint32_t lo16(uint32_t w) { return (w << 4) & 0xF0F0F
 __device__ __forceinline__ uint32_t hi16(uint32_t w) { return w & 0xF0F0F0F0u; }
 __device__ __forceinline__ uint32_t word(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
+// y[m + i, n] for the N sums v (gated: gates v, ups u); rows from `end` on are left alone.  The bias is in the
+// sums already.  All residuals are read before the first value is written: an element is the residual of itself only.
+template <int N, bool GATED>
+__device__ __forceinline__ void finish(const Params& p, long long m, long long end, int n, float (&v)[N], const float (&u)[N]) {
+    float r[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) r[i] = p.residual && m + i < end ? p.residual[(m + i) * p.ldr + n] : 0.f;
+    activate_n(p.act, v);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        if (m + i < end) {
+            float o = GATED ? v[i] * u[i] : v[i];
+            if (p.residual) o += r[i];
+            p.y[(m + i) * p.ldy + n] = o;
+        }
+}
+
 // wk warps, a team, share a unit; blockDim = 32 * wk * (teams of a CTA), and every team has a run of units of its own.
 // WHOLE: K is a multiple of 512; otherwise the groups past the end of a row repeat its last one with scale 0.
 template <bool GATED, bool WHOLE>
@@ -169,10 +186,10 @@ rows_kernel(const Params p, int wk) {
             float v[2] = {acc[0] + ba, acc[1] + ba}, w[2] = {acc[2] + bb, acc[3] + bb};
             if (m < end) {
                 if (GATED) {
-                    if (has_a) finish<2, true>(p, m, 1, end, na, v, w);
+                    if (has_a) finish<2, true>(p, m, end, na, v, w);
                 } else {
-                    if (has_a) finish<2, false>(p, m, 1, end, na, v, v);
-                    if (has_b) finish<2, false>(p, m, 1, end, nb, w, w);
+                    if (has_a) finish<2, false>(p, m, end, na, v, v);
+                    if (has_b) finish<2, false>(p, m, end, nb, w, w);
                 }
             }
         }

@@ -32,13 +32,18 @@ __device__ __forceinline__ float rcp_approx(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
     return d;
 }
+__device__ __forceinline__ float exp_approx(float x) {               // (results below 2^-126 are 0)
+    float d;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x * 1.44269504f));
+    return d;
+}
 // 1 / (1 + exp(-v)): the reciprocal and the power of two to one or two units in the last place
-__device__ __forceinline__ float logistic(float v) { return rcp_approx(1.f + __expf(-v)); }
+__device__ __forceinline__ float logistic(float v) { return rcp_approx(1.f + exp_approx(-v)); }
 // 1 + erf(t), erf by Abramowitz and Stegun 7.1.26 (to 1.5e-7): erfcf takes three times as many instructions, which the tiles,
 // whose accumulators wait meanwhile, spent a third of their time in
 __device__ __forceinline__ float one_plus_erf(float t) {
     const float z = fabsf(t), k = rcp_approx(fmaf(0.3275911f, z, 1.f));
-    const float q = k * fmaf(k, fmaf(k, fmaf(k, fmaf(k, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * __expf(-z * z);
+    const float q = k * fmaf(k, fmaf(k, fmaf(k, fmaf(k, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * exp_approx(-z * z);
     return t < 0.f ? q : 2.f - q;
 }
 template <int ACT>
@@ -65,23 +70,6 @@ __device__ __forceinline__ void activate_n(int act, float (&v)[N]) {
         default: break;
     }
 }
-// y[m + i * step, n] for the N sums v (gated: gates v, ups u); rows from `end` on are left alone.  The bias is in the
-// sums already.  All residuals are read before the first value is written: an element is the residual of itself only.
-template <int N, bool GATED>
-__device__ __forceinline__ void finish(const Params& p, long long m, int step, long long end, int n, float (&v)[N], const float (&u)[N]) {
-    float r[N];
-#pragma unroll
-    for (int i = 0; i < N; i++) r[i] = p.residual && m + i * step < end ? p.residual[(m + i * step) * p.ldr + n] : 0.f;
-    activate_n(p.act, v);
-#pragma unroll
-    for (int i = 0; i < N; i++)
-        if (m + i * step < end) {
-            float o = GATED ? v[i] * u[i] : v[i];
-            if (p.residual) o += r[i];
-            p.y[(m + i * step) * p.ldy + n] = o;
-        }
-}
-
 // A unit is one tile of weight rows times one chunk of a bucket's rows; units of a chunk differ in the tile last.
 struct Unit { int expert, tile, first, count, pad; };
 struct Buckets { int part[33]; };

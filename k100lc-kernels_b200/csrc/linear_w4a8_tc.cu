@@ -10,10 +10,9 @@
 // for two accumulators instead of three.)
 //
 // Roles of the 16 warps of the persistent CTA, joined by mbarriers (every wait is bounded):
-//   * one warp copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring, and the scales of the weight rows
-//     and of the rows of x (cp.async);
+//   * one warp copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring;
 //   * four warps expand them: a thread owns a weight row, reads its 64 bytes and writes 128 to tensor memory, from where
-//     the MMA takes its A operand;
+//     the MMA takes its A operand; it also fetches the scale of its row and of one row of x, some steps ahead;
 //   * one warp copies the rows of x by TMA, put into bucket order and into the k order of the nibbles once per call by a
 //     small kernel in front;
 //   * two warps issue the MMAs of the even and the odd groups, into three accumulators in turn;
@@ -36,19 +35,19 @@ constexpr int RING = 4;                             // stages of A (tensor memor
 constexpr int NACC = 3;                             // accumulators
 constexpr int BP = 8;                               // stages of packed weights
 constexpr int SLOTS = 16;                           // stages of scales (reuse distance: see where they are fetched)
-constexpr int kLag = 6;                             // steps between issuing a fetch of scales and publishing it
+constexpr int kAhead = 6;                           // steps between issuing a fetch of scales and their use
 constexpr int B_BYTES = kCols * 128, BP_BYTES = 128 * 64;
 constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 3, EXP_WARP0 = 4, EPI_WARP0 = 8, kThreads = 16 * 32;
 // 512 threads start with 128 registers each; the shares below add up to no more
 constexpr int kRegsIssue = 72, kRegsExpand = 72, kRegsEpilogue = 184;
 static_assert(kRegsIssue + kRegsExpand + 2 * kRegsEpilogue <= 512, "register shares of the four warpgroups");
-static_assert(SLOTS >= BP + RING + NACC && kLag < BP, "see where the scales are fetched");
+static_assert(SLOTS > kAhead + RING + NACC, "see where the scales are fetched");
 constexpr int kSpin = 1 << 17;
 constexpr uint32_t kTmemCols = 512, kTmemA = NACC * kCols;   // accumulators, then A: 4 x 32 columns
 static_assert(NACC * kCols + RING * 32 <= 512, "tensor memory");
 
 struct __align__(16) Control {
-    uint64_t bp_full[BP], bp_free[BP], s_full[SLOTS];
+    uint64_t bp_full[BP], bp_free[BP];
     uint64_t a_full[RING], b_full[RING], done[RING];
     uint64_t acc_full[2 * NACC], acc_free[2 * NACC], drain[2];
     uint32_t tmem_base;
@@ -138,6 +137,35 @@ struct Ring {
     }
 };
 
+// y[m + i, n] for the N sums v (gated: gates v, ups u); rows from `end` on are left alone.  The bias is in the
+// sums already.  All residuals are read before the first value is written: an element is the residual of itself only.
+template <int N, bool GATED>
+__device__ __forceinline__ void finish_rows(const Params& p, long long m, long long end, int n, float (&v)[N], const float (&u)[N]) {
+    const int left = (int)(end - m);                                 // (a unit has at most 128 rows)
+    float* y = p.y + m * p.ldy + n;
+    activate_n(p.act, v);
+    if (GATED) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] *= u[i];
+    }
+    if (p.residual) {
+        const float* r = p.residual + m * p.ldr + n;
+        float add[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) add[i] = i < left ? r[i * p.ldr] : 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] += add[i];
+    }
+    if (N - 1 < left) {
+#pragma unroll
+        for (int i = 0; i < N; i++) y[i * p.ldy] = v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < left) y[i * p.ldy] = v[i];
+    }
+}
+
 struct RowMaps { CUtensorMap box[4]; };             // boxes of 128, 64, 32 and 16 rows of x (a group)
 
 // GATED: 64 gate rows and 64 up rows make a tile.
@@ -172,7 +200,6 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             mbar_init(&ctl->acc_full[i], 1);
             mbar_init(&ctl->acc_free[i], 4);
         }
-        for (int i = 0; i < SLOTS; i++) mbar_init(&ctl->s_full[i], 1);
         for (int i = 0; i < 2; i++) mbar_init(&ctl->drain[i], 1);
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -187,36 +214,20 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 
     const uint32_t bring_s = smem_u32(bring), wring_s = smem_u32(wring), sring_s = smem_u32(sring), wsring_s = smem_u32(wsring);
     const uint32_t bp_full = smem_u32(ctl->bp_full), bp_free = smem_u32(ctl->bp_free), a_full = smem_u32(ctl->a_full), b_full = smem_u32(ctl->b_full);
-    const uint32_t s_full = smem_u32(ctl->s_full), done = smem_u32(ctl->done), acc_full = smem_u32(ctl->acc_full), acc_free = smem_u32(ctl->acc_free);
+    const uint32_t done = smem_u32(ctl->done), acc_full = smem_u32(ctl->acc_full), acc_free = smem_u32(ctl->acc_free);
     if (warp < EXP_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         // In these roles the whole warp walks the steps and one lane is elected to issue: a single lane that waits alone polls
         // its barrier dozens of times a step, and descriptors stay in uniform registers.
         if (warp == WEIGHT_WARP) {
-            // ================================================================ packed weights and all scales
-            // A lane fetches the scales of four rows of x and the aligned words around those of four weight rows (a copy has at
-            // least four bytes; allocations are whole words).  They are published kLag steps later, when they have landed: two
-            // steps were less than the memory's latency and held the MMAs up.  Step it - BP has been expanded when its weights
-            // are overwritten, so the MMAs up to it - BP - RING have run, which were issued after the accumulators up to step
-            // it - BP - RING - NACC had been drained: nobody reads slot or barrier it % SLOTS any more.
+            // ================================================================ packed weights
             Ring<BP> r;
-            Ring<SLOTS> fetch, behind;
             int it = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const int y0 = un.expert * (GATED ? 2 * p.N : p.N) + un.tile * ROWS, y1 = y0 + (GATED ? p.N : 64);
-                const float* sc[4];
-                uintptr_t wsc[4];
-                bool has[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const long long sr = x_row(p, un, lane + 32 * i);
-                    has[i] = sr >= 0;
-                    sc[i] = p.asc + (sr < 0 ? 0 : (size_t)sr * G);
-                    wsc[i] = reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, lane + 32 * i) * G);
-                }
-                for (int g = 0; g < G; g++, it++, r.next(), fetch.next()) {
+                for (int g = 0; g < G; g++, it++, r.next()) {
                     if (!(ok = wait_warp(bp_free + r.s * 8, r.ph ^ 1, ctl, 21))) break;
                     if (elect_one()) {
                         const uint32_t bar = bp_full + r.s * 8, dst = wring_s + r.s * BP_BYTES;
@@ -225,27 +236,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                         tma_2d_at(dst + BP_BYTES / 2, &map_w, g * 64, y1, bar);
                     }
                     __syncwarp();
-                    const uint32_t slot = fetch.s * 512 + lane * 4;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        cp_async4(sring_s + slot + 128 * i, sc[i], has[i]);
-                        cp_async4(wsring_s + slot + 128 * i, reinterpret_cast<const void*>(wsc[i] & ~(uintptr_t)3), true);
-                        sc[i]++;
-                        wsc[i] += 2;
-                    }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    if (it >= kLag) {
-                        cp_async_wait<kLag>();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_at(s_full + behind.s * 8);
-                        behind.next();
-                    }
                 }
             }
-            cp_async_wait<0>();
-            __syncwarp();
-            if (ok && lane == 0)
-                for (int j = it > kLag ? it - kLag : 0; j < it; j++, behind.next()) mbar_arrive_at(s_full + behind.s * 8);
             if (ctl->abort)                                          // copies in flight land before the memory is given up
                 for (int j = it > BP ? it - BP : 0; j < it; j++)
                     for (int i = 0; i < kSpin && !mbar_try_wait(&ctl->bp_full[j % BP], (j / BP) & 1); i++) {}
@@ -285,20 +277,17 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             const uint32_t par = warp - MMA_WARP;
             const uint64_t bdesc0 = smem_desc_sw128(bring_s);
             Ring<RING> r;
-            Ring<SLOTS> sc;
             Ring<2 * NACC> acc;
             uint32_t parity = 0;                                     // of the first step of the tile
             if (par) {
                 r.next();
-                sc.next();
                 acc.next();
             }
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const uint32_t idesc = instr_desc((un.count + 15) & ~15);
-                for (int g = par ^ parity; g < G; g += 2, r.next2(), sc.next2(), acc.next2()) {
-                    if (!(ok = wait_warp(s_full + sc.s * 8, sc.ph, ctl, 29))) break;     // (for the epilogue)
+                for (int g = par ^ parity; g < G; g += 2, r.next2(), acc.next2()) {
                     if (!(ok = wait_warp(a_full + r.s * 8, r.ph, ctl, 23))) break;
                     if (!(ok = wait_warp(b_full + r.s * 8, r.ph, ctl, 24))) break;
                     const uint32_t late = acc.s >= NACC, d_at = late ? acc.s - NACC : acc.s;
@@ -329,11 +318,45 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         const uint32_t a0 = tmem + ((uint32_t)(q * 32) << 16) + kTmemA;
         const uint32_t x = ((row >> 1) & 3) << 4;                    // 64-byte swizzle: chunk ^= (row / 2) % 4
         const uint32_t w0 = wring_s + row * 64 + x, w1 = wring_s + row * 64 + (16 ^ x), w2 = wring_s + row * 64 + (32 ^ x), w3 = wring_s + row * 64 + (48 ^ x);
+        // A lane fetches the aligned word around the scale of its weight row (a copy has at least four bytes; allocations are
+        // whole words) and the scale of the row of x that is its column, kAhead steps before the expansion that publishes them:
+        // with two steps, less than the memory's latency, the MMAs waited; one warp that fetched for all took 700 clocks a
+        // step.  This warp has seen the MMAs up to step it - 1 - RING done, which were issued after the accumulators up to
+        // it - 1 - RING - NACC had been drained, so nobody reads the slot of step it + kAhead - SLOTS any more.
+        int fu = blockIdx.x, fg = 0;                                 // next to fetch
+        const float* sc = nullptr;
+        uintptr_t wsc = 0;
+        bool has = false;
+        Ring<SLOTS> slot;
+        auto fetch = [&]() {
+            if (fu < total) {
+                if (fg == 0) {
+                    const Unit un = find_unit(p, fu, kCols, tiles, ends);
+                    const long long sr = x_row(p, un, row);
+                    has = sr >= 0;
+                    sc = p.asc + (sr < 0 ? 0 : (size_t)sr * G);
+                    wsc = reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, row) * G);
+                }
+                const uint32_t at = (slot.s * 128 + row) * 4;
+                cp_async4(sring_s + at, sc, has);
+                cp_async4(wsring_s + at, reinterpret_cast<const void*>(wsc & ~(uintptr_t)3), true);
+                sc++;
+                wsc += 2;
+                slot.next();
+                if (++fg == G) {
+                    fg = 0;
+                    fu += gridDim.x;
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        for (int i = 0; i < kAhead; i++) fetch();
         Ring<BP> rp;
         Ring<RING> r;
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
             for (int g = 0; g < G; g++, rp.next(), r.next()) {
+                fetch();
                 if (!(ok = wait_warp(bp_full + rp.s * 8, rp.ph, ctl, 26))) break;
                 const uint32_t at = rp.s * BP_BYTES;
                 const uint4 w[4] = {lds128(w0 + at), lds128(w1 + at), lds128(w2 + at), lds128(w3 + at)};
@@ -349,6 +372,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 }
                 tmem_st32(a0 + r.s * 32, o);
                 tmem_st_wait();
+                cp_async_wait<kAhead>();
                 tc_fence_before();
                 __syncwarp();                                        // (every lane has its words in registers, and A is written)
                 if (lane == 0) {
@@ -357,6 +381,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 }
             }
         }
+        cp_async_wait<0>();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
         // ==================================================================== epilogue
@@ -454,7 +479,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                         v[k] = at[k * 128];
                         up[k] = GATED ? at[k * 128 + 64] : 0.f;
                     }
-                    finish<4, GATED>(p, m, 1, end, n, v, up);
+                    finish_rows<4, GATED>(p, m, end, n, v, up);
                 }
             int all;
             asm volatile("{\n.reg .pred p, q;\nsetp.ne.s32 p, %1, 0;\nbar.red.and.pred q, 1, 256, p;\nselp.s32 %0, 1, 0, q;\n}" : "=r"(all) : "r"((int)ok) : "memory");
