@@ -41,7 +41,7 @@ constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 3, EXP_WARP0 = 4, EPI_WA
 // 512 threads start with 128 registers each; the shares below add up to no more
 constexpr int kRegsIssue = 72, kRegsExpand = 72, kRegsEpilogue = 184;
 static_assert(kRegsIssue + kRegsExpand + 2 * kRegsEpilogue <= 512, "register shares of the four warpgroups");
-static_assert(SLOTS > kAhead + RING + NACC, "see where the scales are fetched");
+static_assert(SLOTS > kAhead + RING + NACC + 1, "see where the scales are fetched");
 constexpr int kSpin = 1 << 17;
 constexpr uint32_t kTmemCols = 512, kTmemA = NACC * kCols;   // accumulators, then A: 4 x 32 columns
 static_assert(NACC * kCols + RING * 32 <= 512, "tensor memory");
@@ -80,26 +80,33 @@ __device__ __forceinline__ void expand_word(uint32_t w, uint32_t* o) {
     o[1] = w & 0xF0F0F0F0u;
 }
 
-// codes [xrows][K/2] even and odd -> [m][K] in that order; slot s of a plan takes row bucket_rows[s].  A thread moves 32 k;
-// slots behind the last bucket and slots of no row are skipped.
+// Codes [xrows][K/2] even and odd -> [m][K] in that order, scales [xrows][K/128] -> [K/128][m]; slot s of a plan takes row
+// bucket_rows[s], and scale 0 if there is no such row.  A thread moves 32 k of a row and a scale at a time; slots behind the
+// last bucket are skipped.
 __global__ void __launch_bounds__(256)
-order_codes_kernel(const Params p, int8_t* __restrict__ out) {
+order_codes_kernel(const Params p, int8_t* __restrict__ out, float* __restrict__ scales) {
     pdl_wait();
-    const int per_row = p.K / 32;
-    const long long used = p.offsets ? bound(p, p.n_exp) : p.m, n = used * per_row;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const long long slot = i / per_row;
+    const int per_row = p.K / 32, G = p.K / 128;
+    const long long used = p.offsets ? bound(p, p.n_exp) : p.m, n = used * per_row, n_scales = used * G;
+    const long long first = (long long)blockIdx.x * blockDim.x + threadIdx.x, step = (long long)gridDim.x * blockDim.x;
+    auto row_of = [&](long long slot) -> long long {
+        if (!p.bucket_rows) return slot;
+        const int row = p.bucket_rows[slot];
+        return row >= 0 && row < p.xrows ? row : -1;
+    };
+    for (long long i = first; i < n; i += step) {
+        const long long slot = i / per_row, row = row_of(slot);
         const int c = (int)(i - slot * per_row);
-        long long row = slot;
-        if (p.bucket_rows) {
-            row = p.bucket_rows[slot];
-            if (row < 0 || row >= p.xrows) continue;
-        }
+        if (row < 0) continue;
         const uint4 e = *reinterpret_cast<const uint4*>(p.ae + row * (p.K / 2) + c * 16);
         const uint4 o = *reinterpret_cast<const uint4*>(p.ao + row * (p.K / 2) + c * 16);
         uint4* dst = reinterpret_cast<uint4*>(out + slot * p.K + c * 32);
         dst[0] = make_uint4(e.x, o.x, e.y, o.y);
         dst[1] = make_uint4(e.z, o.z, e.w, o.w);
+    }
+    for (long long i = first; i < n_scales; i += step) {
+        const long long g = i / used, slot = i - g * used, row = row_of(slot);
+        scales[g * p.m + slot] = row < 0 ? 0.f : p.asc[row * G + g];
     }
     pdl_launch_dependents();
 }
@@ -171,7 +178,7 @@ struct RowMaps { CUtensorMap box[4]; };             // boxes of 128, 64, 32 and 
 // GATED: 64 gate rows and 64 up rows make a tile.
 template <bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
-tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ RowMaps map_x, const Params p) {
+tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ RowMaps map_x, const float* __restrict__ scales, const Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* bring = smem;                                           // RING x [128 rows][128 bytes]
@@ -318,11 +325,12 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         const uint32_t a0 = tmem + ((uint32_t)(q * 32) << 16) + kTmemA;
         const uint32_t x = ((row >> 1) & 3) << 4;                    // 64-byte swizzle: chunk ^= (row / 2) % 4
         const uint32_t w0 = wring_s + row * 64 + x, w1 = wring_s + row * 64 + (16 ^ x), w2 = wring_s + row * 64 + (32 ^ x), w3 = wring_s + row * 64 + (48 ^ x);
-        // A lane fetches the aligned word around the scale of its weight row (a copy has at least four bytes; allocations are
-        // whole words) and the scale of the row of x that is its column, kAhead steps before the expansion that publishes them:
-        // with two steps, less than the memory's latency, the MMAs waited; one warp that fetched for all took 700 clocks a
-        // step.  This warp has seen the MMAs up to step it - 1 - RING done, which were issued after the accumulators up to
-        // it - 1 - RING - NACC had been drained, so nobody reads the slot of step it + kAhead - SLOTS any more.
+        // A lane fetches the scale of the row of x that is its column and the aligned word around the scale of its weight row,
+        // kAhead steps before the expansion that publishes them.  (A copy has at least four bytes, two groups; a lane copies
+        // each word once, into the slot of the step that first needs it.  Allocations are whole words.)  With two steps, less
+        // than the memory's latency, the MMAs waited; one warp that fetched for all took 700 clocks a step.
+        // This warp has seen the MMAs up to step it - 1 - RING done, which were issued after the accumulators up to step
+        // it - 1 - RING - NACC had been drained, so nobody reads the slot of step it + kAhead - SLOTS or the one before any more.
         int fu = blockIdx.x, fg = 0;                                 // next to fetch
         const float* sc = nullptr;
         uintptr_t wsc = 0;
@@ -332,15 +340,14 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             if (fu < total) {
                 if (fg == 0) {
                     const Unit un = find_unit(p, fu, kCols, tiles, ends);
-                    const long long sr = x_row(p, un, row);
-                    has = sr >= 0;
-                    sc = p.asc + (sr < 0 ? 0 : (size_t)sr * G);
+                    has = (int)row < un.count;
+                    sc = scales + un.first + (has ? row : 0);
                     wsc = reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, row) * G);
                 }
                 const uint32_t at = (slot.s * 128 + row) * 4;
                 cp_async4(sring_s + at, sc, has);
-                cp_async4(wsring_s + at, reinterpret_cast<const void*>(wsc & ~(uintptr_t)3), true);
-                sc++;
+                if (fg == 0 || !(wsc & 2)) cp_async4(wsring_s + at, reinterpret_cast<const void*>(wsc & ~(uintptr_t)3), true);
+                sc += p.m;
                 wsc += 2;
                 slot.next();
                 if (++fg == G) {
@@ -413,7 +420,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 if (!(ok = wait_warp(acc_full + acc.s * 8, acc.ph, ctl, 28))) break;
                 tc_fence_after();
                 const uint32_t slot = r.s * 512, sb = sring_s + slot, d = d0 + (acc.s >= NACC ? acc.s - NACC : acc.s) * kCols;
-                const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(lds32(sw0 + slot) >> shift))) * 0.0625f);
+                const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((unsigned short)(lds32(sw0 + (g && shift ? (r.s - 1) % SLOTS * 512 : slot)) >> shift))) * 0.0625f);
                 const uint64_t s2 = pack2(s, s);
 #pragma unroll
                 for (int a = 0; a < 8; a++) {
@@ -499,9 +506,10 @@ size_t smem_bytes(const Params& p) {
 }  // namespace
 
 int run_tiles(const char* kn, const LaunchCtx& c, const Params& p) {
-    const size_t bytes = (size_t)p.m * p.K;
+    const size_t codes = (size_t)p.m * p.K, bytes = codes + (size_t)p.m * (p.K / 128) * 4;
     int8_t* xq = static_cast<int8_t*>(engine_scratch(bytes));
     FM_REQUIRE(xq, kn, "the engine workspace cannot grow to %zu bytes here (inside a capture: raise FM_SCRATCH_MB)", bytes);
+    float* scales = reinterpret_cast<float*>(xq + codes);
     CUtensorMap map_w;
     RowMaps map_x;
     const uint64_t wrows = (uint64_t)p.n_exp * p.N * (p.gated ? 2 : 1);
@@ -511,7 +519,7 @@ int run_tiles(const char* kn, const LaunchCtx& c, const Params& p) {
     const size_t n = (size_t)p.m * (p.K / 32);
     size_t eb = (n + 255) / 256;
     if (eb > (size_t)c.sm_count * 16) eb = (size_t)c.sm_count * 16;
-    cudaError_t e = launch_kernel(order_codes_kernel, dim3((unsigned)eb), dim3(256), 0, c.stream, pdl_enabled(), p, xq);
+    cudaError_t e = launch_kernel(order_codes_kernel, dim3((unsigned)eb), dim3(256), 0, c.stream, pdl_enabled(), p, xq, scales);
     if (e != cudaSuccess) return cuda_fail(kn, e);
     const int rc = after_launch(kn);
     if (rc != FM_OK) return rc;
@@ -524,7 +532,7 @@ int run_tiles(const char* kn, const LaunchCtx& c, const Params& p) {
     const long long units = chunks * ((p.N + rows - 1) / rows);
     FM_REQUIRE(units < (1ll << 30), kn, "%lld tiles are too many for one call", units);
     const unsigned grid = (unsigned)(units < c.sm_count ? units : c.sm_count);
-    e = launch_kernel(kern, dim3(grid), dim3(kThreads), smem, c.stream, pdl_enabled(), map_w, map_x, p);
+    e = launch_kernel(kern, dim3(grid), dim3(kThreads), smem, c.stream, pdl_enabled(), map_w, map_x, static_cast<const float*>(scales), p);
     return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
 }
 
