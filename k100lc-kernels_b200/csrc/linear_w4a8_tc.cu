@@ -71,6 +71,13 @@ __device__ __forceinline__ bool wait_warp(uint32_t b, uint32_t parity, Control* 
     return __all_sync(0xffffffffu, wait(b, parity, ctl, code));
 }
 
+// two barriers in the time of one when both are ready
+__device__ __forceinline__ bool wait_warp2(uint32_t b0, uint32_t parity0, int code0, uint32_t b1, uint32_t parity1, int code1, Control* ctl) {
+    const bool r0 = mbar_try_wait_at(b0, parity0), r1 = mbar_try_wait_at(b1, parity1);
+    if (__all_sync(0xffffffffu, r0 && r1)) return true;
+    return wait_warp(b0, parity0, ctl, code0) && wait_warp(b1, parity1, ctl, code1);
+}
+
 // kind::i8: s32 accumulator, s8 operands, both K-major, M = 128
 __device__ __forceinline__ uint32_t instr_desc(int n) { return 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24; }
 
@@ -295,8 +302,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 const Unit un = find_unit(p, u, kCols, tiles, ends);
                 const uint32_t idesc = instr_desc((un.count + 15) & ~15);
                 for (int g = par ^ parity; g < G; g += 2, r.next2(), acc.next2()) {
-                    if (!(ok = wait_warp(a_full + r.s * 8, r.ph, ctl, 23))) break;
-                    if (!(ok = wait_warp(b_full + r.s * 8, r.ph, ctl, 24))) break;
+                    if (!(ok = wait_warp2(a_full + r.s * 8, r.ph, 23, b_full + r.s * 8, r.ph, 24, ctl))) break;
                     const uint32_t late = acc.s >= NACC, d_at = late ? acc.s - NACC : acc.s;
                     if (!(ok = wait_warp(acc_free + (late ? d_at : d_at + NACC) * 8, acc.ph ^ 1 ^ late, ctl, 22))) break;
                     tc_fence_after();
@@ -363,11 +369,9 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
             for (int g = 0; g < G; g++, rp.next(), r.next()) {
-                fetch();
-                if (!(ok = wait_warp(bp_full + rp.s * 8, rp.ph, ctl, 26))) break;
+                if (!(ok = wait_warp2(bp_full + rp.s * 8, rp.ph, 26, done + r.s * 8, r.ph ^ 1, 27, ctl))) break;
                 const uint32_t at = rp.s * BP_BYTES;
                 const uint4 w[4] = {lds128(w0 + at), lds128(w1 + at), lds128(w2 + at), lds128(w3 + at)};
-                if (!(ok = wait_warp(done + r.s * 8, r.ph ^ 1, ctl, 27))) break;
                 tc_fence_after();
                 uint32_t o[32];
 #pragma unroll
@@ -378,8 +382,9 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                     expand_word(w[j].w, o + 8 * j + 6);
                 }
                 tmem_st32(a0 + r.s * 32, o);
-                tmem_st_wait();
+                fetch();
                 cp_async_wait<kAhead>();
+                tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();                                        // (every lane has its words in registers, and A is written)
                 if (lane == 0) {
