@@ -202,11 +202,12 @@ rows_kernel(const Params p, int wk) {
     pdl_launch_dependents();
 }
 
-cudaError_t run_rows(const LaunchCtx& c, const Params& p) {
+int run_rows(const char* kn, const LaunchCtx& c, const Params& p) {
     const int rows = p.gated ? 8 : 16, tiles = (p.N + rows - 1) / rows, parts = (p.K / 128 + CH - 1) / CH;
     long long chunks = (p.m + COLS - 1) / COLS;
     if (p.offsets) chunks = p.n_exp < p.m ? chunks + p.n_exp : p.m;   // every bucket may end in a part of a chunk
     const long long units = chunks * tiles, slots = (long long)c.sm_count * kCtasPerSm * kMaxWarps;
+    FM_REQUIRE(units < (1ll << 30), kn, "%lld tiles are too many for one call", units);
     // the K dimension is split over warps while all of them stay resident at once and each keeps a chunk
     int wk = (int)(slots / units < kMaxWarps ? slots / units : kMaxWarps);
     if (wk > parts) wk = parts;
@@ -217,16 +218,29 @@ cudaError_t run_rows(const LaunchCtx& c, const Params& p) {
     const size_t smem = p.offsets ? (size_t)p.n_exp * 4 : 0;
     const bool whole = p.K % 512 == 0;
     auto kern = p.gated ? (whole ? rows_kernel<true, true> : rows_kernel<true, false>) : (whole ? rows_kernel<false, true> : rows_kernel<false, false>);
-    return launch_kernel(kern, dim3((unsigned)grid), dim3(wk * per_cta * 32), smem, c.stream, pdl_enabled(), p, wk);
-}
-
-int run(const char* kn, const LaunchCtx& c, const Params& p) {
-    // rows per bucket, were all experts equally popular
-    const int per = p.offsets ? p.m / (p.n_exp < p.m ? p.n_exp : p.m) : p.m;
-    if (per > 16) return run_tiles(kn, c, p);
-    const cudaError_t e = run_rows(c, p);
+    const cudaError_t e = launch_kernel(kern, dim3((unsigned)grid), dim3(wk * per_cta * 32), smem, c.stream, pdl_enabled(), p, wk);
     return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
 }
+
+// Rows or tiles, whichever promises to be done first.  The rows kernel reads the weights of a bucket once for every 8 rows, at
+// 5.6 MB a microsecond and more; a tile takes 0.35 us for a 128-group, one wave of tiles after the other, 2.5 us later than
+// the rows kernel starts.  (Buckets as if all experts were equally popular, half a piece added for the rest of each.)
+// Measured, rows against tiles: 17408 x 5120 at 16 rows 19.0 and 22.3 us, at 17 rows 27.3 and 23.1; 5120 x 17408 at 32 rows 53.8
+// and 54.6; 2048 x 2048 at 48 rows 8.1 and 13.8; 8 of 64 gated experts of 1024 x 5120 at 72 tokens 94 and 109, at 128 142
+// and 114.
+bool rows_first(const LaunchCtx& c, const Params& p) {
+    const long long used = !p.offsets ? 1 : p.n_exp < p.m ? p.n_exp : p.m, rows = p.gated ? 64 : 128;
+    auto pieces = [&](int of) {
+        if (!p.offsets) return (p.m + of - 1ll) / of;
+        const long long n = p.m / of + used / 2;
+        return n < used ? used : n;
+    };
+    const double bytes = (double)pieces(COLS) * p.N * (p.gated ? p.K : p.K / 2);
+    const long long tiles = pieces(128) * ((p.N + rows - 1) / rows), steps = (tiles + c.sm_count - 1) / c.sm_count * (p.K / 128);
+    return bytes <= 2e6 * (7 + steps);
+}
+
+int run(const char* kn, const LaunchCtx& c, const Params& p) { return rows_first(c, p) ? run_rows(kn, c, p) : run_tiles(kn, c, p); }
 
 // what both entries check: weights, codes of `xrows` rows, `m` output rows
 int check(const char* kn, const Params& p, int n_exp, long long xrows) {

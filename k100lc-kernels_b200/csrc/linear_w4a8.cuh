@@ -71,21 +71,26 @@ __device__ __forceinline__ void activate_n(int act, float (&v)[N]) {
     }
 }
 // A unit is one tile of weight rows times one chunk of a bucket's rows; units of a chunk differ in the tile last.
-struct Unit { int expert, tile, first, count, pad; };
+struct Unit { int expert, tile, first, count; };
 struct Buckets { int part[33]; };
 
-// bounds of bucket e, held to [0, m]: a damaged plan cannot lead out of the output
+// bounds of bucket e, held to [0, m]
 __device__ __forceinline__ int bound(const Params& p, int e) { return min(max(p.offsets[e], 0), p.m); }
 
-// Number of units; ends[e] becomes the number of units of the experts up to e.  All threads of the CTA call it.
+// Number of units; ends[e] becomes the number of units of the experts up to e.  0 for a damaged plan (bounds that fall or lie
+// outside of [0, m]): nothing is read or written by it.  All threads of the CTA call it.
 __device__ __forceinline__ int count_units(const Params& p, int cols, int tiles, int* ends, Buckets* bk) {
     if (!p.offsets) return (p.m + cols - 1) / cols * tiles;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    int carry = 0;
+    int carry = 0, damaged = 0;
     for (int e0 = 0; e0 < p.n_exp; e0 += blockDim.x) {
         const int e = e0 + (int)threadIdx.x;
         int v = 0;
-        if (e < p.n_exp) v = (max(bound(p, e + 1) - bound(p, e), 0) + cols - 1) / cols * tiles;
+        if (e < p.n_exp) {
+            const int lo = p.offsets[e], hi = p.offsets[e + 1];
+            damaged |= lo < 0 || hi < lo || hi > p.m;
+            v = damaged ? 0 : (hi - lo + cols - 1) / cols * tiles;
+        }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int t = __shfl_up_sync(0xffffffffu, v, o);
@@ -102,8 +107,7 @@ __device__ __forceinline__ int count_units(const Params& p, int cols, int tiles,
         if (e < p.n_exp) ends[e] = carry + v;
         carry += all;
     }
-    __syncthreads();
-    return carry;
+    return __syncthreads_or(damaged) ? 0 : carry;
 }
 
 // TILE_LAST: the units of a bucket walk its chunks of rows first (they share a tile of weights), otherwise its tiles first
@@ -129,7 +133,6 @@ __device__ __forceinline__ Unit find_unit_by(const Params& p, int u, int cols, i
     r.tile = TILE_LAST ? i : j;
     r.first = begin + (TILE_LAST ? j : i) * cols;
     r.count = min(cols, end - r.first);
-    r.pad = 0;
     return r;
 }
 

@@ -611,7 +611,9 @@ plan_place_kernel(const int* __restrict__ ids, float* __restrict__ w, int* __res
 }
 
 // ------------------------------------------------------------------------------------------------------- host side
-constexpr int kFusePairs = 4096;                    // placed by one block: 1.6 us for 384 pairs, a launch costs about as much
+// Pairs that the last block of the routing places itself, instead of a second launch: 256 experts, 8 choices, in us for 384
+// pairs 8.9 against 12.5, for 1024 10.6 against 11.8, for 2048 14.1 against 11.8.
+constexpr int kFusePairs = 1024;
 constexpr int kFuseExperts = 256;
 
 template <typename T>
