@@ -34,6 +34,7 @@ def _dense(rt, m, n, k, act="none", gated=False, bias=False, residual=False, see
         out = pr if in_place else bf.zeros(m * ldy, np.float32, -777.0)
         lin.forward_codes_device([bf.put(c) for c in cd], m, residual_dev=pr, out_dev=out, ldy=ldy, ldr=ldr)
         got = bf.get(out, m * ldy).reshape(m, ldy)
+        assert rt.gemm_status() == 0
         lin.ws.free()
     if not in_place:
         assert np.all(got[:, n:] == -777.0)
@@ -68,6 +69,46 @@ def test_dense_model_shapes(rt, m, n, k):
     _dense(rt, m, n, k, "gelu", bias=True)
 
 
+# From here to the experts: enough rows and weights for the tensor-core tiles.  One group and odd numbers of groups, rows of
+# weights and of x that end inside a tile, more tiles than an SM (so that a CTA walks several).
+@pytest.mark.parametrize("m,n,k", [(300, 1000, 5120), (700, 1000, 1152), (4100, 129, 1152), (3000, 1000, 128), (129, 17408, 1152), (65, 17407, 1280),
+                                   (2049, 1300, 384)])
+def test_tiles_sizes(rt, m, n, k):
+    _dense(rt, m, n, k)
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_tiles_epilogue(rt, act, gated):
+    _dense(rt, 1030, 700, 1152, act, gated, bias=True, residual=True)
+    _dense(rt, 1030, 700, 1152, act, gated, bias=True, seed=1)
+    _dense(rt, 1030, 700, 1152, act, gated, residual=True, seed=2)
+
+
+def test_tiles_row_strides_and_residual_in_place(rt):
+    _dense(rt, 1030, 700, 1152, "silu", bias=True, residual=True, ldy=711, ldr=705)
+    _dense(rt, 1030, 700, 1152, "silu", residual=True, in_place=True)
+    _dense(rt, 1030, 700, 1152, "silu", residual=True, in_place=True, ldy=703, ldr=703, gated=True)
+
+
+@pytest.mark.parametrize("m,n,k,gated", [(513, 5000, 640, False), (513, 2500, 640, True), (1000, 5000, 128, False), (300, 17408, 5120, False)])
+def test_tiles_repeat_bit_for_bit(rt, m, n, k, gated):
+    """Forty calls in a row: a role that gets ahead of another would show as another sum or as a wait that ran out."""
+    rng = np.random.default_rng(m)
+    wq, ws, _ = P.layer(rng, 1, n * (2 if gated else 1), k)
+    cd, _ = P.codes(rng, m, k)
+    with Bufs(rt) as b:
+        lin = FusedLinear(rt, n, k, b.put(wq), b.put(ws), act="silu", gated=gated)
+        dev, outs = [b.put(c) for c in cd], [b.zeros(m * n) for _ in range(2)]
+        lin.forward_codes_device(dev, m, out_dev=outs[0])
+        first = b.get(outs[0], m * n)
+        for i in range(40):
+            lin.forward_codes_device(dev, m, out_dev=outs[1])
+            if i % 8 == 7:
+                assert np.array_equal(b.get(outs[1], m * n), first)
+        assert rt.gemm_status() == 0
+
+
 def test_dense_is_the_by_name_layer(rt):
     """Without an epilogue the layer is RT4Linear's: both sum the same exact integers, in another order."""
     rng = np.random.default_rng(8)
@@ -99,6 +140,7 @@ def _experts(rt, rows, n_exp, topk, n, k, act="none", gated=False, bias=False, g
         out = bf.zeros(max(1, rows * topk * n), np.float32, -777.0)
         lin.forward_codes_device([bf.put(c) for c in cd], plan, gather=gather, out_dev=out)
         got = bf.get(out, rows * topk * n).reshape(rows * topk, n)
+        assert rt.gemm_status() == 0
         lin.ws.free()
     assert np.all(got[total:] == -777.0)
     for e in range(n_exp):
@@ -115,6 +157,39 @@ def _experts(rt, rows, n_exp, topk, n, k, act="none", gated=False, bias=False, g
 def test_experts_sizes(rt, rows, n_exp, topk, n, k, gather):
     _experts(rt, rows, n_exp, topk, n, k, gather=gather)
     _experts(rt, rows, n_exp, topk, n, k, "silu", True, True, gather)
+
+
+@pytest.mark.parametrize("rows,n_exp,topk,n,k", [(2000, 5, 2, 130, 1152), (1500, 16, 4, 257, 1152), (1999, 24, 4, 600, 640)])
+@pytest.mark.parametrize("gather", [False, True])
+def test_experts_tiles(rt, rows, n_exp, topk, n, k, gather):
+    _experts(rt, rows, n_exp, topk, n, k, gather=gather)
+    _experts(rt, rows, n_exp, topk, n // 2, k, "silu", True, True, gather)
+
+
+def test_experts_tiles_uneven_buckets(rt):
+    """Empty experts at both ends and between, buckets of one row and of hundreds, pairs without an expert."""
+    rng = np.random.default_rng(3)
+    ids = rng.choice([-1, 2, 3, 7, 38], p=[0.1, 0.6, 0.001, 0.199, 0.1], size=(3000, 1))
+    for gather in (False, True):
+        _experts(rt, 3000, 40, 1, 300, 1152, "gelu", bias=True, gather=gather, ids=ids)
+    _experts(rt, 3000, 40, 1, 300, 1152, ids=np.full((3000, 1), -1))
+
+
+@pytest.mark.parametrize("rows,n,k", [(16, 40, 256), (3000, 300, 1152)])
+def test_experts_damaged_plan_writes_nothing(rt, rows, n, k):
+    rng = np.random.default_rng(rows)
+    wq, ws, _ = P.layer(rng, 3, n, k)
+    cd, _ = P.codes(rng, rows, k)
+    with Bufs(rt) as b:
+        lin = ExpertLinear(rt, 3, n, k, b.put(wq), b.put(ws))
+        codes, none = [b.put(c) for c in cd], b.zeros(rows, np.int32)
+        for bounds in ([0, 9, 4, rows], [-1, 3, 5, rows], [0, 3, 5, rows + 1], [0, -2 ** 31, 2 ** 31 - 1, rows], [7, 7, 7, 7]):
+            plan = MoEPlan(rows=rows, topk=1, n_exp=3, ids=0, weights=0, bucket_rows=none, base=0, offsets=b.put(np.array(bounds, np.int32)))
+            for gather in (False, True):
+                out = b.zeros(rows * n, np.float32, -777.0)
+                lin.forward_codes_device(codes, plan, gather=gather, out_dev=out)
+                assert np.all(b.get(out, rows * n) == -777.0)
+        assert rt.gemm_status() == 0
 
 
 def test_experts_uneven_buckets(rt):

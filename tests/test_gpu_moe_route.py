@@ -110,6 +110,40 @@ def test_route_resolves_keys_that_fp32_cannot(rt):
             _check(got, values, **kw)
 
 
+@pytest.mark.parametrize("rows", [5, 128, 129, 600])
+@pytest.mark.parametrize("n_exp", [16, 300])
+def test_route_alone_is_route_with_plan(rt, rows, n_exp):
+    """moe_route_k, then moe_plan_k: what the one call gives on either side of its choice of one launch or two."""
+    x = np.random.default_rng(rows).standard_normal((rows, n_exp)).astype(np.float32)
+    got, values = _run(rt, x, topk=8, score="sigmoid")
+    _check(got, values, topk=8, score="sigmoid")
+    with Bufs(rt) as b:
+        ids, w, slot, base, off = b.zeros(rows * 8, np.int32), b.zeros(rows * 8), b.zeros(rows * 8, np.int32), b.zeros(rows * 8, np.int32), b.zeros(n_exp + 1, np.int32)
+        rt.launch("moe_route_k", 1, 1, [b.put(x), 0, ids, w, rows, n_exp, 8, 1, 1, 1, 1, 1, 1.0, 0])
+        rt.launch("moe_plan_k", 1, 1, [ids, w, slot, base, off, rows, n_exp, 8])
+        assert np.array_equal(b.get(ids, rows * 8, np.int32), got["ids"].reshape(-1)) and np.array_equal(b.get(w, rows * 8), got["w"].reshape(-1))
+        assert np.array_equal(b.get(slot, rows * 8, np.int32), got["bucket"]) and np.array_equal(b.get(base, rows * 8, np.int32), got["base"].reshape(-1))
+        assert np.array_equal(b.get(off, n_exp + 1, np.int32), got["offsets"])
+
+
+def test_routes_back_to_back(rt):
+    """Routers of both kinds in turn, without a wait between them: they share the engine's workspace and a counter."""
+    rng = np.random.default_rng(9)
+    xs = [rng.standard_normal((r, 24)).astype(np.float32) for r in (1, 700, 40, 1999, 3, 512)]
+    with Workspace(rt) as ws:
+        routers = [MoERouter(rt, 24, 2, ws=ws, tag=f"r{i}") for i in range(len(xs))]
+        px = [ws.upload(f"x{i}", x) for i, x in enumerate(xs)]
+        for _ in range(20):
+            plans = [r.forward_device(p, x.shape[0]) for r, p, x in zip(routers, px, xs)]
+        rt.sync()
+        for plan, x in zip(plans, xs):
+            n = x.shape[0] * 2
+            got = dict(ids=rt.download(plan.ids, n, np.int32).reshape(-1, 2), w=rt.download(plan.weights, n, np.float32).reshape(-1, 2),
+                       bucket=rt.download(plan.bucket_rows, n, np.int32), base=rt.download(plan.base, n, np.int32).reshape(-1, 2),
+                       offsets=rt.download(plan.offsets, 25, np.int32))
+            _check(got, x, topk=2)
+
+
 def test_route_no_rows(rt):
     got, _ = _run(rt, np.zeros((0, 8), np.float32), topk=2)
     assert np.array_equal(got["offsets"], np.zeros(9, np.int32))
@@ -142,6 +176,12 @@ def test_route_and_plan_refuse(rt):
             with pytest.raises(RuntimeError, match="rejected"):
                 rt.launch("moe_route_k", 1, 1, ok[:at] + [bad] + ok[at + 1:])
         bucket, base, off = b.zeros(16, np.int32), b.zeros(16, np.int32), b.zeros(9, np.int32)
+        both = ok[:4] + [bucket, base, off] + ok[4:]
+        rt.launch("moe_route_plan_k", 1, 1, both)
+        for at, bad in ((7, -1), (7, 9), (8, 0), (8, 1025), (8, 9), (9, 0), (9, 9), (10, 3), (11, 2), (12, 0), (13, 2), (14, 2), (16, 3), (0, x + 2),
+                        (0, x + 4), (1, x + 240), (2, ids + 4), (3, w + 4), (4, bucket + 4), (4, 0), (5, base + 2), (6, off + 4)):
+            with pytest.raises(RuntimeError, match="rejected"):
+                rt.launch("moe_route_plan_k", 1, 1, both[:at] + [bad] + both[at + 1:])
         ok = [ids, w, bucket, base, off, 8, 8, 2]
         rt.launch("moe_plan_k", 1, 1, ok)
         for at, bad in ((5, -1), (5, 9), (6, 0), (6, 9), (6, 1025), (7, 0), (7, 33), (0, ids + 4), (1, 0), (2, bucket + 4), (3, base + 2), (4, off + 4)):
