@@ -88,34 +88,27 @@ __device__ __forceinline__ void expand_word(uint32_t w, uint32_t* o) {
 }
 
 // Codes [xrows][K/2] even and odd -> [m][K] in that order, scales [xrows][K/128] -> [K/128][m]; slot s of a plan takes row
-// bucket_rows[s], and scale 0 if there is no such row.  A thread moves 32 k of a row and a scale at a time; slots behind the
-// last bucket are skipped.
+// bucket_rows[s], and scale 0 if there is no such row.  A thread moves 32 k of a row, one in four of them the scale of the group
+// too; slots behind the last bucket are skipped.  (The tiles are launched meanwhile, as far as their first wait.)
 __global__ void __launch_bounds__(256)
 order_codes_kernel(const Params p, int8_t* __restrict__ out, float* __restrict__ scales) {
     pdl_wait();
-    const int per_row = p.K / 32, G = p.K / 128;
-    const long long used = p.offsets ? bound(p, p.n_exp) : p.m, n = used * per_row, n_scales = used * G;
-    const long long first = (long long)blockIdx.x * blockDim.x + threadIdx.x, step = (long long)gridDim.x * blockDim.x;
-    auto row_of = [&](long long slot) -> long long {
-        if (!p.bucket_rows) return slot;
-        const int row = p.bucket_rows[slot];
-        return row >= 0 && row < p.xrows ? row : -1;
-    };
-    for (long long i = first; i < n; i += step) {
-        const long long slot = i / per_row, row = row_of(slot);
-        const int c = (int)(i - slot * per_row);
-        if (row < 0) continue;
+    pdl_launch_dependents();
+    const unsigned per_row = p.K / 32, G = p.K / 128;
+    const long long n = (long long)(p.offsets ? bound(p, p.n_exp) : p.m) * per_row;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+        const long long slot = n < (1ll << 32) ? (unsigned)i / per_row : i / per_row;
+        const unsigned c = (unsigned)(i - slot * per_row);
+        const long long row = p.bucket_rows ? p.bucket_rows[slot] : slot;
+        const bool is = !p.bucket_rows || (row >= 0 && row < p.xrows);
+        if (c % 4 == 0) scales[(size_t)(c / 4) * p.m + slot] = is ? p.asc[row * G + c / 4] : 0.f;
+        if (!is) continue;
         const uint4 e = *reinterpret_cast<const uint4*>(p.ae + row * (p.K / 2) + c * 16);
         const uint4 o = *reinterpret_cast<const uint4*>(p.ao + row * (p.K / 2) + c * 16);
         uint4* dst = reinterpret_cast<uint4*>(out + slot * p.K + c * 32);
         dst[0] = make_uint4(e.x, o.x, e.y, o.y);
         dst[1] = make_uint4(e.z, o.z, e.w, o.w);
     }
-    for (long long i = first; i < n_scales; i += step) {
-        const long long g = i / used, slot = i - g * used, row = row_of(slot);
-        scales[g * p.m + slot] = row < 0 ? 0.f : p.asc[row * G + g];
-    }
-    pdl_launch_dependents();
 }
 
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool take) {
@@ -537,7 +530,7 @@ int run_tiles(const char* kn, const LaunchCtx& c, const Params& p) {
     const long long units = chunks * ((p.N + rows - 1) / rows);
     FM_REQUIRE(units < (1ll << 30), kn, "%lld tiles are too many for one call", units);
     const unsigned grid = (unsigned)(units < c.sm_count ? units : c.sm_count);
-    e = launch_kernel(kern, dim3(grid), dim3(kThreads), smem, c.stream, pdl_enabled(), map_w, map_x, static_cast<const float*>(scales), p);
+    e = launch_kernel(kern, dim3(grid), dim3(kThreads), smem, c.stream, true, map_w, map_x, static_cast<const float*>(scales), p);
     return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
 }
 

@@ -570,10 +570,10 @@ plan_count_kernel(const int* __restrict__ ids, const float* __restrict__ w, int*
     pdl_launch_dependents();
 }
 
+// Launched while the kernel in front ends (what that writes is read through no path that may be read ahead of pdl_wait).
 // Every block adds up the counts of all blocks (blockDim / n_exp threads to an expert) and places its own pairs.
 __global__ void __launch_bounds__(1024)
-plan_place_kernel(const int* __restrict__ ids, float* __restrict__ w, int* __restrict__ bucket_rows, int* __restrict__ base,
-                  int* __restrict__ offsets, const int* __restrict__ hist, int pairs, int n_exp, int topk, int per_block) {
+plan_place_kernel(const int* ids, float* w, int* __restrict__ bucket_rows, int* __restrict__ base, int* __restrict__ offsets, const int* hist, int pairs, int n_exp, int topk, int per_block) {
     extern __shared__ int sm[];
     int* total = sm;                                                  // [n_exp]
     int* first = sm + n_exp;                                          // [n_exp] first the pairs of earlier blocks
@@ -588,7 +588,7 @@ plan_place_kernel(const int* __restrict__ ids, float* __restrict__ w, int* __res
         int all = 0, before = 0;
 #pragma unroll 16
         for (int b = s; b < blocks; b += split) {
-            const int h = __ldg(hist + (size_t)b * n_exp + e);
+            const int h = __ldcg(hist + (size_t)b * n_exp + e);
             all += h;
             if (b < (int)blockIdx.x) before += h;
         }
@@ -645,7 +645,7 @@ int run_place(const char* kn, const LaunchCtx& c, const int* ids, float* w, int*
         const cudaError_t e = cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return cuda_fail(kn, e);
     }
-    const cudaError_t e = launch_kernel(plan_place_kernel, dim3(blocks), dim3(1024), smem, c.stream, pdl_enabled(), ids, w, bucket_rows, base, offsets, hist,
+    const cudaError_t e = launch_kernel(plan_place_kernel, dim3(blocks), dim3(1024), smem, c.stream, true, ids, w, bucket_rows, base, offsets, hist,
                                         pairs, n_exp, topk, per_block);
     return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
 }
