@@ -54,7 +54,10 @@ struct __align__(16) Control {
     volatile int abort;
 };
 
-__device__ int g_status;                            // 0, or the code 21.. of the first bounded wait that ran out
+// 0, or the code of the first bounded wait that ran out: 21 packed stage not free, 22 accumulator not drained, 23 weights not
+// expanded, 24 rows of x not landed, 25 and 27 step not done (copy, expansion), 26 packed weights not landed, 28 accumulator
+// not complete.  Read and cleared by fm_gemm_status().
+__device__ int g_status;
 
 __device__ __forceinline__ bool wait(uint32_t b, uint32_t parity, Control* ctl, int code) {
     for (int i = 0; i < kSpin; i++) {

@@ -555,7 +555,7 @@ route_kernel(const RouteParams p, int tokens, bool fuse) {
 
 // hist[block][n_exp] of pairs that are given
 __global__ void __launch_bounds__(kThreads)
-plan_count_kernel(const int* __restrict__ ids, const float* __restrict__ w, int* __restrict__ hist, int pairs, int n_exp, int per_block) {
+plan_count_kernel(const int* ids, const float* w, int* hist, int pairs, int n_exp, int per_block) {
     extern __shared__ int count[];
     pdl_wait();
     for (int e = threadIdx.x; e < n_exp; e += kThreads) count[e] = 0;

@@ -231,8 +231,8 @@ class ExpertLinear(_Product):
 class MoEMLP:
     """Mixture-of-experts feed-forward block ``y[t] = sum_j w[t, j] * down_e(act(gate_e(x_t)) * up_e(x_t))`` with
     e = ids[t, j]: router, one gated product over all buckets, quantiser, one down product, weighted combine — seven
-    launches whatever the number of experts, none of them waiting for the host, so that the block can be
-    captured into a graph.  ``gate_up`` is a gated ``ExpertLinear``, ``down`` a plain one."""
+    launches for a few tokens, ten for many, whatever the number of experts, none of them waiting for the host, so
+    that the block can be captured into a graph (after a first call with as many rows, which sizes the buffers).  ``gate_up`` is a gated ``ExpertLinear``, ``down`` a plain one."""
 
     def __init__(self, rt: Runtime, router: MoERouter, gate_up: ExpertLinear, down: ExpertLinear, ws: Workspace | None = None,
                  tag: str | None = None):
