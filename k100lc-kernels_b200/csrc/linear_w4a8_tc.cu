@@ -147,35 +147,6 @@ struct Ring {
     }
 };
 
-// y[m + i, n] for the N sums v (gated: gates v, ups u); rows from `end` on are left alone.  The bias is in the
-// sums already.  All residuals are read before the first value is written: an element is the residual of itself only.
-template <int N, bool GATED>
-__device__ __forceinline__ void finish_rows(const Params& p, long long m, long long end, int n, float (&v)[N], const float (&u)[N]) {
-    const int left = (int)(end - m);                                 // (a unit has at most 128 rows)
-    float* y = p.y + m * p.ldy + n;
-    activate_n(p.act, v);
-    if (GATED) {
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] *= u[i];
-    }
-    if (p.residual) {
-        const float* r = p.residual + m * p.ldr + n;
-        float add[N];
-#pragma unroll
-        for (int i = 0; i < N; i++) add[i] = i < left ? r[i * p.ldr] : 0.f;
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] += add[i];
-    }
-    if (N - 1 < left) {
-#pragma unroll
-        for (int i = 0; i < N; i++) y[i * p.ldy] = v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            if (i < left) y[i * p.ldy] = v[i];
-    }
-}
-
 struct RowMaps { CUtensorMap box[4]; };             // boxes of 128, 64, 32 and 16 rows of x (a group)
 
 // GATED: 64 gate rows and 64 up rows make a tile.
@@ -451,6 +422,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             // wait takes part in the barriers all the same; the last one of the tile tells all.
             const int t = threadIdx.x & 127;
             const long long end = (long long)un.first + un.count;
+            auto first_of = [&](int i) { return (long long)un.first + ((i & 48) * 2 + set * 16 + (i & 15)); };      // row of sum i
 #pragma unroll
             for (int a = 0; a < 8; a += 2) {                         // (by static index: C stays in registers)
                 if (a >= chunks) break;
@@ -475,20 +447,58 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             }
             if (GATED) asm volatile("bar.sync %0, 128;" ::"r"(2 + set) : "memory");          // gate lane gr meets up lane 64 + gr
             const int n = n0 + (GATED ? t & 63 : (int)row);
-            if (n < p.N)
+            if (n < p.N) {
+                float* sums = mine + n - n0;
+                const bool keep = p.residual != nullptr;             // (for the loop below)
 #pragma unroll 1
-                for (int i = GATED ? t >> 6 << 2 : 0; i < 64; i += GATED ? 8 : 4) {
-                    const long long m = (long long)un.first + ((i & 48) * 2 + set * 16 + (i & 15));
+                for (int i = GATED ? t >> 6 << 2 : 0; i < 64 && (GATED || !keep || p.act); i += GATED ? 8 : 4) {
+                    const long long m = first_of(i);
                     if (m >= end) break;
-                    const float* at = mine + i * 128 + n - n0;
-                    float v[4], up[4];
+                    float v[4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        v[k] = at[k * 128];
-                        up[k] = GATED ? at[k * 128 + 64] : 0.f;
+                    for (int k = 0; k < 4; k++) v[k] = sums[(i + k) * 128];
+                    activate_n(p.act, v);
+                    if (GATED) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) v[k] *= sums[(i + k) * 128 + 64];
                     }
-                    finish_rows<4, GATED>(p, m, end, n, v, up);
+                    if (keep) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) sums[(i + k) * 128] = v[k];
+                    } else {
+                        const int left = (int)(end - m);
+                        float* y = p.y + m * p.ldy + n;
+                        if (left >= 4) {
+#pragma unroll
+                            for (int k = 0; k < 4; k++) y[k * p.ldy] = v[k];
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 3; k++)
+                                if (k < left) y[k * p.ldy] = v[k];
+                        }
+                    }
                 }
+                // the residual in a loop of its own, 16 or 8 loads on their way: one latency a row of four was twice the products'
+                // time at 1228 x 10187 x 1536.  An element is the residual of itself only, read by the thread that writes it.
+                if (keep) {
+                    constexpr int AT_ONCE = GATED ? 8 : 16;
+#pragma unroll 1
+                    for (int i = 0; i < 64; i += 16) {
+                        const long long m = first_of(i);
+                        const int left = (int)(end - m);
+                        if (left <= 0) break;
+                        const float* r = p.residual + m * p.ldr + n;
+                        float* y = p.y + m * p.ldy + n;
+                        auto at = [&](int j) { return GATED ? (j >> 2) * 8 + (t >> 6) * 4 + (j & 3) : j; };
+                        float add[AT_ONCE];
+#pragma unroll
+                        for (int j = 0; j < AT_ONCE; j++) add[j] = at(j) < left ? r[at(j) * p.ldr] : 0.f;
+#pragma unroll
+                        for (int j = 0; j < AT_ONCE; j++)
+                            if (at(j) < left) y[at(j) * p.ldy] = sums[(i + at(j)) * 128] + add[j];
+                    }
+                }
+            }
             int all;
             asm volatile("{\n.reg .pred p, q;\nsetp.ne.s32 p, %1, 0;\nbar.red.and.pred q, 1, 256, p;\nselp.s32 %0, 1, 0, q;\n}" : "=r"(all) : "r"((int)ok) : "memory");
             if (!all) break;
