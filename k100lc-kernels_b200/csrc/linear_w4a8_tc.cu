@@ -451,29 +451,29 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 float* sums = mine + n - n0;
                 const bool keep = p.residual != nullptr;             // (for the loop below)
 #pragma unroll 1
-                for (int i = GATED ? t >> 6 << 2 : 0; i < 64 && (GATED || !keep || p.act); i += GATED ? 8 : 4) {
+                for (int i = GATED ? t >> 6 << 3 : 0; i < 64 && (GATED || !keep || p.act); i += GATED ? 16 : 8) {
                     const long long m = first_of(i);
                     if (m >= end) break;
-                    float v[4];
+                    float v[8];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) v[k] = sums[(i + k) * 128];
+                    for (int k = 0; k < 8; k++) v[k] = sums[(i + k) * 128];
                     activate_n(p.act, v);
                     if (GATED) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++) v[k] *= sums[(i + k) * 128 + 64];
+                        for (int k = 0; k < 8; k++) v[k] *= sums[(i + k) * 128 + 64];
                     }
                     if (keep) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++) sums[(i + k) * 128] = v[k];
+                        for (int k = 0; k < 8; k++) sums[(i + k) * 128] = v[k];
                     } else {
                         const int left = (int)(end - m);
                         float* y = p.y + m * p.ldy + n;
-                        if (left >= 4) {
+                        if (left >= 8) {
 #pragma unroll
-                            for (int k = 0; k < 4; k++) y[k * p.ldy] = v[k];
+                            for (int k = 0; k < 8; k++) y[k * p.ldy] = v[k];
                         } else {
 #pragma unroll
-                            for (int k = 0; k < 3; k++)
+                            for (int k = 0; k < 7; k++)
                                 if (k < left) y[k * p.ldy] = v[k];
                         }
                     }
@@ -489,7 +489,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                         if (left <= 0) break;
                         const float* r = p.residual + m * p.ldr + n;
                         float* y = p.y + m * p.ldy + n;
-                        auto at = [&](int j) { return GATED ? (j >> 2) * 8 + (t >> 6) * 4 + (j & 3) : j; };
+                        auto at = [&](int j) { return GATED ? (t >> 6) * 8 + j : j; };
                         float add[AT_ONCE];
 #pragma unroll
                         for (int j = 0; j < AT_ONCE; j++) add[j] = at(j) < left ? r[at(j) * p.ldr] : 0.f;

@@ -87,6 +87,7 @@ def test_tiles_epilogue(rt, act, gated):
 
 def test_tiles_row_strides_and_residual_in_place(rt):
     _dense(rt, 1030, 700, 1152, "silu", bias=True, residual=True, ldy=711, ldr=705)
+    _dense(rt, 1030, 700, 1152, residual=True, in_place=True)
     _dense(rt, 1030, 700, 1152, "silu", residual=True, in_place=True)
     _dense(rt, 1030, 700, 1152, "silu", residual=True, in_place=True, ldy=703, ldr=703, gated=True)
 
