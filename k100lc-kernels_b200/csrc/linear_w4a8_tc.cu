@@ -451,29 +451,29 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 float* sums = mine + n - n0;
                 const bool keep = p.residual != nullptr;             // (for the loop below)
 #pragma unroll 1
-                for (int i = GATED ? t >> 6 << 3 : 0; i < 64 && (GATED || !keep || p.act); i += GATED ? 16 : 8) {
+                for (int i = GATED ? t >> 6 << 4 : 0; i < 64 && (GATED || !keep || p.act); i += GATED ? 32 : 16) {
                     const long long m = first_of(i);
                     if (m >= end) break;
-                    float v[8];
+                    float v[16];
 #pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] = sums[(i + k) * 128];
+                    for (int k = 0; k < 16; k++) v[k] = sums[(i + k) * 128];
                     activate_n(p.act, v);
                     if (GATED) {
 #pragma unroll
-                        for (int k = 0; k < 8; k++) v[k] *= sums[(i + k) * 128 + 64];
+                        for (int k = 0; k < 16; k++) v[k] *= sums[(i + k) * 128 + 64];
                     }
                     if (keep) {
 #pragma unroll
-                        for (int k = 0; k < 8; k++) sums[(i + k) * 128] = v[k];
+                        for (int k = 0; k < 16; k++) sums[(i + k) * 128] = v[k];
                     } else {
                         const int left = (int)(end - m);
                         float* y = p.y + m * p.ldy + n;
-                        if (left >= 8) {
+                        if (left >= 16) {
 #pragma unroll
-                            for (int k = 0; k < 8; k++) y[k * p.ldy] = v[k];
+                            for (int k = 0; k < 16; k++) y[k * p.ldy] = v[k];
                         } else {
 #pragma unroll
-                            for (int k = 0; k < 7; k++)
+                            for (int k = 0; k < 15; k++)
                                 if (k < left) y[k * p.ldy] = v[k];
                         }
                     }
@@ -481,21 +481,20 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 // the residual in a loop of its own, 16 or 8 loads on their way: one latency a row of four was twice the products'
                 // time at 1228 x 10187 x 1536.  An element is the residual of itself only, read by the thread that writes it.
                 if (keep) {
-                    constexpr int AT_ONCE = GATED ? 8 : 16;
+                    constexpr int AT_ONCE = 16;
 #pragma unroll 1
-                    for (int i = 0; i < 64; i += 16) {
+                    for (int i = GATED ? t >> 6 << 4 : 0; i < 64; i += GATED ? 32 : 16) {
                         const long long m = first_of(i);
                         const int left = (int)(end - m);
                         if (left <= 0) break;
                         const float* r = p.residual + m * p.ldr + n;
                         float* y = p.y + m * p.ldy + n;
-                        auto at = [&](int j) { return GATED ? (t >> 6) * 8 + j : j; };
                         float add[AT_ONCE];
 #pragma unroll
-                        for (int j = 0; j < AT_ONCE; j++) add[j] = at(j) < left ? r[at(j) * p.ldr] : 0.f;
+                        for (int j = 0; j < AT_ONCE; j++) add[j] = j < left ? r[j * p.ldr] : 0.f;
 #pragma unroll
                         for (int j = 0; j < AT_ONCE; j++)
-                            if (at(j) < left) y[at(j) * p.ldy] = sums[(i + at(j)) * 128] + add[j];
+                            if (j < left) y[j * p.ldy] = sums[(i + j) * 128] + add[j];
                     }
                 }
             }
