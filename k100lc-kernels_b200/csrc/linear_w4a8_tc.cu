@@ -42,6 +42,7 @@ constexpr int WEIGHT_WARP = 0, MMA_WARP = 1, ROW_WARP = 3, EXP_WARP0 = 4, EPI_WA
 constexpr int kRegsIssue = 72, kRegsExpand = 72, kRegsEpilogue = 184;
 static_assert(kRegsIssue + kRegsExpand + 2 * kRegsEpilogue <= 512, "register shares of the four warpgroups");
 static_assert(SLOTS > kAhead + RING + NACC + 1, "see where the scales are fetched");
+constexpr int kOutPitch = 68;                       // values between weight rows of the sums on their way out (16-byte words, no two of eight rows in a bank)
 constexpr int kSpin = 1 << 17;
 constexpr uint32_t kTmemCols = 512, kTmemA = NACC * kCols;   // accumulators, then A: 4 x 32 columns
 static_assert(NACC * kCols + RING * 32 <= 512, "tensor memory");
@@ -159,8 +160,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
     uint8_t* wring = bring + RING * B_BYTES;                         // BP x [128 rows][64 bytes]
     float* sring = reinterpret_cast<float*>(wring + BP * BP_BYTES);  // SLOTS x [128]
     uint32_t* wsring = reinterpret_cast<uint32_t*>(sring + SLOTS * kCols);   // SLOTS x [128]: the word that holds the weight row's scale
-    float* xch = reinterpret_cast<float*>(wsring + SLOTS * 128);     // a set's [64 columns][128 rows] of sums on their way out, twice
-    Control* ctl = reinterpret_cast<Control*>(xch + 128 * 128);
+    float* xch = reinterpret_cast<float*>(wsring + SLOTS * 128);     // a set's [128 rows][64 columns] of sums on their way out, twice
+    Control* ctl = reinterpret_cast<Control*>(xch + 2 * 128 * kOutPitch);
     int* ends = reinterpret_cast<int*>(ctl + 1);                     // [n_exp]
     __shared__ Buckets bk;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -368,7 +369,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         // waits, loads and sums; a tile's two partial sums meet on their way out.  warp: lanes 32 q .. of the accumulators
         const uint32_t set = (warp - EPI_WARP0) >> 2, q = warp & 3, row = q * 32 + lane;
         const uint32_t d0 = tmem + ((uint32_t)(q * 32) << 16), sw0 = wsring_s + row * 4;
-        float *const mine = xch + set * (64 * 128), *const theirs = xch + (set ^ 1) * (64 * 128);
+        float *const mine = xch + set * (128 * kOutPitch), *const theirs = xch + (set ^ 1) * (128 * kOutPitch);
         Ring<SLOTS> r;
         Ring<2 * NACC> acc;
         uint32_t parity = 0;                                         // of the first step of the tile
@@ -427,28 +428,25 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             for (int a = 0; a < 8; a += 2) {                         // (by static index: C stays in registers)
                 if (a >= chunks) break;
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint64_t c = set ? C[a][j] : C[a + 1][j];
-                    theirs[(a * 8 + 2 * j) * 128 + row] = __uint_as_float((uint32_t)c);
-                    theirs[(a * 8 + 2 * j + 1) * 128 + row] = __uint_as_float((uint32_t)(c >> 32));
-                }
+                for (int j = 0; j < 8; j += 2)
+                    *reinterpret_cast<ulonglong2*>(theirs + row * kOutPitch + a * 8 + 2 * j) = make_ulonglong2(set ? C[a][j] : C[a + 1][j], set ? C[a][j + 1] : C[a + 1][j + 1]);
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
+            const uint64_t bias2 = pack2(__float_as_uint(bias), __float_as_uint(bias));
 #pragma unroll
             for (int a = 0; a < 8; a += 2) {
                 if (a >= chunks) break;
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint64_t c = set ? C[a + 1][j] : C[a][j];
-                    float* at = mine + (a * 8 + 2 * j) * 128 + row;
-                    at[0] += __uint_as_float((uint32_t)c) + bias;
-                    at[128] += __uint_as_float((uint32_t)(c >> 32)) + bias;
+                for (int j = 0; j < 8; j += 2) {
+                    ulonglong2* at = reinterpret_cast<ulonglong2*>(mine + row * kOutPitch + a * 8 + 2 * j);
+                    const ulonglong2 o = *at;
+                    *at = make_ulonglong2(add2p(o.x, add2p(set ? C[a + 1][j] : C[a][j], bias2)), add2p(o.y, add2p(set ? C[a + 1][j + 1] : C[a][j + 1], bias2)));
                 }
             }
             if (GATED) asm volatile("bar.sync %0, 128;" ::"r"(2 + set) : "memory");          // gate lane gr meets up lane 64 + gr
             const int n = n0 + (GATED ? t & 63 : (int)row);
             if (n < p.N) {
-                float* sums = mine + n - n0;
+                float* sums = mine + (n - n0) * kOutPitch;
                 const bool keep = p.residual != nullptr;             // (for the loop below)
 #pragma unroll 1
                 for (int i = GATED ? t >> 6 << 4 : 0; i < 64 && (GATED || !keep || p.act); i += GATED ? 32 : 16) {
@@ -456,15 +454,15 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                     if (m >= end) break;
                     float v[16];
 #pragma unroll
-                    for (int k = 0; k < 16; k++) v[k] = sums[(i + k) * 128];
+                    for (int k = 0; k < 16; k++) v[k] = sums[i + k];
                     activate_n(p.act, v);
                     if (GATED) {
 #pragma unroll
-                        for (int k = 0; k < 16; k++) v[k] *= sums[(i + k) * 128 + 64];
+                        for (int k = 0; k < 16; k++) v[k] *= sums[64 * kOutPitch + i + k];
                     }
                     if (keep) {
 #pragma unroll
-                        for (int k = 0; k < 16; k++) sums[(i + k) * 128] = v[k];
+                        for (int k = 0; k < 16; k++) sums[i + k] = v[k];
                     } else {
                         const int left = (int)(end - m);
                         float* y = p.y + m * p.ldy + n;
@@ -478,10 +476,9 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                         }
                     }
                 }
-                // the residual in a loop of its own, 16 or 8 loads on their way: one latency a row of four was twice the products'
+                // the residual in a loop of its own, 16 loads on their way: one latency for every four rows was twice the products'
                 // time at 1228 x 10187 x 1536.  An element is the residual of itself only, read by the thread that writes it.
                 if (keep) {
-                    constexpr int AT_ONCE = 16;
 #pragma unroll 1
                     for (int i = GATED ? t >> 6 << 4 : 0; i < 64; i += GATED ? 32 : 16) {
                         const long long m = first_of(i);
@@ -489,12 +486,12 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                         if (left <= 0) break;
                         const float* r = p.residual + m * p.ldr + n;
                         float* y = p.y + m * p.ldy + n;
-                        float add[AT_ONCE];
+                        float add[16];
 #pragma unroll
-                        for (int j = 0; j < AT_ONCE; j++) add[j] = j < left ? r[j * p.ldr] : 0.f;
+                        for (int j = 0; j < 16; j++) add[j] = j < left ? r[j * p.ldr] : 0.f;
 #pragma unroll
-                        for (int j = 0; j < AT_ONCE; j++)
-                            if (j < left) y[j * p.ldy] = sums[(i + j) * 128] + add[j];
+                        for (int j = 0; j < 16; j++)
+                            if (j < left) y[j * p.ldy] = sums[i + j] + add[j];
                     }
                 }
             }
@@ -510,7 +507,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 }
 
 size_t smem_bytes(const Params& p) {
-    return 1024 + RING * B_BYTES + BP * BP_BYTES + SLOTS * (kCols + 128) * 4 + 128 * 128 * 4 + sizeof(Control) + (size_t)p.n_exp * 4;
+    return 1024 + RING * B_BYTES + BP * BP_BYTES + SLOTS * (kCols + 128) * 4 + 2 * 128 * kOutPitch * 4 + sizeof(Control) + (size_t)p.n_exp * 4;
 }
 
 }  // namespace
