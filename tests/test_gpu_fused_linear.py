@@ -110,6 +110,48 @@ def test_tiles_repeat_bit_for_bit(rt, m, n, k, gated):
         assert rt.gemm_status() == 0
 
 
+def test_tiles_and_placement_in_graphs(rt):
+    """Two captured runs of a router of many tokens and of products on tiles, replayed in turn with other inputs: the graphs
+    share the engine's workspace, and each holds launches that begin while the one in front ends."""
+    rng = np.random.default_rng(6)
+    rows, n_exp, n, k = 900, 6, 600, 1152
+    wq, ws, w = P.layer(rng, n_exp, n, k)
+    with Bufs(rt) as b:
+        router = [MoERouter(rt, n_exp, 2) for _ in range(2)]
+        experts = ExpertLinear(rt, n_exp, n, k, b.put(wq), b.put(ws))
+        dense = FusedLinear(rt, n, k, experts.wq, experts.ws_scale, act="silu")
+        px, pl = b.zeros(rows * k), b.zeros(rows * n_exp)
+        pe, pd = [b.zeros(rows * 2 * n) for _ in range(2)], [b.zeros(rows * n) for _ in range(2)]
+
+        def queue(i):
+            plan = router[i].forward_device(pl, rows)
+            experts.forward_device(px, plan, out_dev=pe[i])
+            dense.forward_device(px, rows, out_dev=pd[i])
+            return plan
+
+        plans = [queue(i) for i in range(2)]                       # sizes the workspaces
+        graphs = []
+        for i in range(2):
+            rt.graph_begin()
+            queue(i)
+            graphs.append(rt.graph_end())
+        for _ in range(3):
+            rt.upload(px, rng.standard_normal((rows, k)).astype(np.float32))
+            logits = rng.standard_normal((rows, n_exp)).astype(np.float32)
+            rt.upload(pl, logits)
+            for g in graphs:
+                rt.graph_launch(g)
+            got = [(b.get(pe[i], rows * 2 * n), b.get(pd[i], rows * n), b.get(plans[i].offsets, n_exp + 1, np.int32)) for i in range(2)]
+            for x, y in zip(*got):
+                assert np.array_equal(x, y)
+            assert np.array_equal(got[0][2], P.plan(*P.route(logits, 2), n_exp)[3])
+            queue(0)
+            assert np.array_equal(b.get(pe[0], rows * 2 * n), got[0][0]) and np.array_equal(b.get(pd[0], rows * n), got[0][1])
+        assert rt.gemm_status() == 0
+        for g in graphs:
+            rt.graph_free(g)
+
+
 def test_dense_is_the_by_name_layer(rt):
     """Without an epilogue the layer is RT4Linear's: both sum the same exact integers, in another order."""
     rng = np.random.default_rng(8)
