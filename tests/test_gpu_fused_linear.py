@@ -209,6 +209,10 @@ def test_experts_tiles(rt, rows, n_exp, topk, n, k, gather):
     _experts(rt, rows, n_exp, topk, n // 2, k, "silu", True, True, gather)
 
 
+def test_experts_tiles_most_experts(rt):
+    _experts(rt, 20000, 1024, 2, 129, 640, bias=True)
+
+
 def test_experts_tiles_uneven_buckets(rt):
     """Empty experts at both ends and between, buckets of one row and of hundreds, pairs without an expert."""
     rng = np.random.default_rng(3)
