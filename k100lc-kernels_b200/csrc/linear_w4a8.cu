@@ -21,8 +21,8 @@
 // Bound by HBM.  A warp asks for a group of its next chunk (four groups: 256 bytes of every row) as soon as it has multiplied
 // that group of the current one, so that 4 KB a warp are on their way at any time, across the ends of its units too.  Where
 // there are fewer units than warps the K dimension is split over the warps of a team and their partial sums meet in shared
-// memory.  Measured (B200, cold weights): one row of 17408 x 5120 12.3 us (10.9 in a graph, 4.2 TB/s; 8 rows 11.8), five rows of
-// 5120 x 17408 18.6 us, 33 tokens through 8 of 64 experts of 5120 x 1024 40.5 us (4.4 TB/s, 0.67 of a copy's rate): what is left
+// memory.  Measured (B200, cold weights): one row of 17408 x 5120 12.3 us (11.0 in a graph, 4.2 TB/s; 8 rows 11.9), five rows of
+// 5120 x 17408 18.1 us (16.0), 33 tokens through 8 of 64 experts of 5120 x 1024 39.5 us (4.5 TB/s, 0.68 of a copy's rate): what is left
 // is the time from a launch to the first weights and the last unit's tail.
 #include <cuda_fp16.h>
 
@@ -210,8 +210,10 @@ int run_rows(const char* kn, const LaunchCtx& c, const Params& p) {
     if (p.offsets) chunks = p.n_exp < p.m ? chunks + p.n_exp : p.m;   // every bucket may end in a part of a chunk
     const long long units = chunks * tiles, slots = (long long)c.sm_count * kCtasPerSm * kMaxWarps;
     FM_REQUIRE(units < (1ll << 30), kn, "%lld tiles are too many for one call", units);
-    // the K dimension is split over warps while all of them stay resident at once and each keeps a chunk
+    // the K dimension is split over warps while all of them stay resident at once, each keeps a chunk and every team has one
+    // unit at most (320 units of 5120 x 17408, 5 rows: 17.1 us with 7 warps a team, of which 24 of 296 had two units, 16.2 with 4)
     int wk = (int)(slots / units < kMaxWarps ? slots / units : kMaxWarps);
+    while (wk > 1 && (long long)c.sm_count * kCtasPerSm * (kMaxWarps / wk) < units) wk--;
     if (wk > parts) wk = parts;
     if (wk < 1) wk = 1;
     const int per_cta = kMaxWarps / wk;
