@@ -13,8 +13,8 @@
 //   * one warp copies packed weight tiles (128 rows x 64 bytes, two TMA boxes) into a ring;
 //   * four warps expand them: a thread owns a weight row, reads its 64 bytes and writes 128 to tensor memory, from where
 //     the MMA takes its A operand; it also fetches the scale of its row and of one row of x, some steps ahead;
-//   * one warp copies the rows of x by TMA, put into bucket order and into the k order of the nibbles once per call by a
-//     small kernel in front;
+//   * one warp copies the rows of x by TMA, put into bucket order by a small kernel in front, or their even and odd codes from
+//     where they are;
 //   * two warps issue the MMAs of the even and the odd groups, into three accumulators in turn;
 //   * eight warps, four for the even and four for the odd groups, drain the accumulators: C[m, n] = fmaf(float(I), ws * asc,
 //     C) in registers, then the epilogue.
@@ -93,15 +93,17 @@ __device__ __forceinline__ bool wait_warp2(uint32_t b0, uint32_t parity0, int co
 // kind::i8: s32 accumulator, s8 operands, both K-major, M = 128
 __device__ __forceinline__ uint32_t instr_desc(int n) { return 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24; }
 
-// Eight two's-complement nibbles of a word -> 16 times their value as bytes, k0,k2,k4,k6 and k1,k3,k5,k7.
+// Eight two's-complement nibbles of a word -> 16 times their value as bytes, the even k of a group before the odd ones, as the
+// codes of x are stored.
 __device__ __forceinline__ void expand_word(uint32_t w, uint32_t* o) {
     o[0] = (w << 4) & 0xF0F0F0F0u;
-    o[1] = w & 0xF0F0F0F0u;
+    o[16] = w & 0xF0F0F0F0u;
 }
 
-// Codes [xrows][K/2] even and odd -> [m][K] in that order, scales [xrows][K/128] -> [K/128][m]; slot s of a plan takes row
-// bucket_rows[s], and scale 0 if there is no such row.  A thread moves 32 k of a row, one in four of them the scale of the group
-// too; slots behind the last bucket are skipped.  (The tiles are launched meanwhile, as far as their first wait.)
+// Rows of x into bucket order, [m][K] with the even codes of a group before its odd ones, and their scales, [K/128][m]; slot s
+// of a plan takes row bucket_rows[s], and scale 0 if there is no such row.  A thread moves 32 k of a row, one in four of them
+// the scale of the group too; slots behind the last bucket are skipped.  (The tiles are launched meanwhile, as far as their first
+// wait.)
 __global__ void __launch_bounds__(256)
 order_codes_kernel(const Params p, int8_t* __restrict__ out, float* __restrict__ scales) {
     pdl_wait();
@@ -115,11 +117,9 @@ order_codes_kernel(const Params p, int8_t* __restrict__ out, float* __restrict__
         const bool is = !p.bucket_rows || (row >= 0 && row < p.xrows);
         if (c % 4 == 0) scales[(size_t)(c / 4) * p.m + slot] = is ? p.asc[row * G + c / 4] : 0.f;
         if (!is) continue;
-        const uint4 e = *reinterpret_cast<const uint4*>(p.ae + row * (p.K / 2) + c * 16);
-        const uint4 o = *reinterpret_cast<const uint4*>(p.ao + row * (p.K / 2) + c * 16);
-        uint4* dst = reinterpret_cast<uint4*>(out + slot * p.K + c * 32);
-        dst[0] = make_uint4(e.x, o.x, e.y, o.y);
-        dst[1] = make_uint4(e.z, o.z, e.w, o.w);
+        int8_t* dst = out + slot * p.K + c / 4 * 128 + c % 4 * 16;
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(p.ae + row * (p.K / 2) + c * 16);
+        *reinterpret_cast<uint4*>(dst + 64) = *reinterpret_cast<const uint4*>(p.ao + row * (p.K / 2) + c * 16);
     }
 }
 
@@ -156,15 +156,17 @@ struct Ring {
     }
 };
 
-struct RowMaps { CUtensorMap box[4]; };             // boxes of 128, 64, 32 and 16 rows of x (a group)
+// boxes of 128, 64, 32 and 16 rows of x: a group's codes put in order, or (direct) its even and its odd ones from where they are
+struct RowMaps { CUtensorMap box[4], odd[4]; };
+struct Scales { const float* at; long long row, group; };            // of slot s and group g: at[s * row + g * group]
 
 // GATED: 64 gate rows and 64 up rows make a tile.
 template <bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
-tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ RowMaps map_x, const float* __restrict__ scales, const Params p) {
+tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ RowMaps map_x, const Scales scales, const bool direct, const Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t* bring = smem;                                           // RING x [128 rows][128 bytes]
+    uint8_t* bring = smem;                                           // RING x [128 rows][128 bytes], or even and odd codes [128 rows][64 bytes]
     uint8_t* wring = bring + RING * B_BYTES;                         // BP x [128 rows][64 bytes]
     float* sring = reinterpret_cast<float*>(wring + BP * BP_BYTES);  // SLOTS x [128]
     uint32_t* wsring = reinterpret_cast<uint32_t*>(sring + SLOTS * kCols);   // SLOTS x [128]: the word that holds the weight row's scale
@@ -235,6 +237,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
             // ================================================================ rows of x
             // A count of rows is a sum of boxes of 128, 64, 32 and 16: a box costs its issue, about 100 clocks, whatever it holds
             // (16-row boxes throughout, 16 instructions a step, bound the tile at 1800 clocks; four-row gathers at 6000).
+            const int width = direct ? 64 : 128;
             Ring<RING> r;
             int it = 0;
             bool ok = true;
@@ -251,9 +254,10 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
 #pragma unroll
                         for (int b = 0; b < 4; b++)
                             if (n16 & (128 >> b)) {
-                                tma_2d_at(dst, &map_x.box[b], g * 128, at, bar);
+                                tma_2d_at(dst, &map_x.box[b], g * width, at, bar);
+                                if (direct) tma_2d_at(dst + B_BYTES / 2, &map_x.odd[b], g * width, at, bar);
                                 at += 128 >> b;
-                                dst += (128 >> b) * 128;
+                                dst += (128 >> b) * width;
                             }
                     }
                     __syncwarp();
@@ -265,7 +269,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
         } else {
             // ================================================================ MMA issuers: even and odd steps
             const uint32_t par = warp - MMA_WARP;
-            const uint64_t bdesc0 = smem_desc_sw128(bring_s);
+            const uint64_t bdesc0 = direct ? smem_desc_sw64(bring_s) : smem_desc_sw128(bring_s);
+            const uint32_t odd = direct ? B_BYTES / 2 >> 4 : 64 >> 4;
             Ring<RING> r;
             Ring<2 * NACC> acc;
             uint32_t parity = 0;                                     // of the first step of the tile
@@ -287,7 +292,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                     if (elect_one()) {
 #pragma unroll
                         for (int j = 0; j < 4; j++)                  // 32 k each: 8 columns of A, 32 bytes of B
-                            tc_mma_i8_ts(d, a + j * 8, bd + j * 2, idesc, j > 0);
+                            tc_mma_i8_ts(d, a + j * 8, bd + (j >> 1) * odd + (j & 1) * 2, idesc, j > 0);
                         tc_commit_at(acc_full + acc.s * 8);
                         tc_commit_at(done + r.s * 8);
                     }
@@ -323,13 +328,13 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 if (fg == 0) {
                     const Unit un = find_unit(p, fu, kCols, tiles, ends);
                     has = (int)row < un.count;
-                    sc = scales + un.first + (has ? row : 0);
+                    sc = scales.at + (un.first + (has ? (long long)row : 0)) * scales.row;
                     wsc = reinterpret_cast<uintptr_t>(p.ws + weight_row<GATED>(p, un, row) * G);
                 }
                 const uint32_t at = (slot.s * 128 + row) * 4;
                 cp_async4(sring_s + at, sc, has);
                 if (fg == 0 || !(wsc & 2)) cp_async4(wsring_s + at, reinterpret_cast<const void*>(wsc & ~(uintptr_t)3), true);
-                sc += p.m;
+                sc += scales.group;
                 wsc += 2;
                 slot.next();
                 if (++fg == G) {
@@ -352,10 +357,10 @@ tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ R
                 uint32_t o[32];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    expand_word(w[j].x, o + 8 * j);
-                    expand_word(w[j].y, o + 8 * j + 2);
-                    expand_word(w[j].z, o + 8 * j + 4);
-                    expand_word(w[j].w, o + 8 * j + 6);
+                    expand_word(w[j].x, o + 4 * j);
+                    expand_word(w[j].y, o + 4 * j + 1);
+                    expand_word(w[j].z, o + 4 * j + 2);
+                    expand_word(w[j].w, o + 4 * j + 3);
                 }
                 tmem_st32(a0 + r.s * 32, o);
                 fetch();
@@ -521,33 +526,47 @@ size_t smem_bytes(const Params& p) {
 }  // namespace
 
 int run_tiles(const char* kn, const LaunchCtx& c, const Params& p) {
-    const size_t codes = (size_t)p.m * p.K, bytes = codes + (size_t)p.m * (p.K / 128) * 4;
-    int8_t* xq = static_cast<int8_t*>(engine_scratch(bytes));
-    FM_REQUIRE(xq, kn, "the engine workspace cannot grow to %zu bytes here (inside a capture: raise FM_SCRATCH_MB)", bytes);
-    float* scales = reinterpret_cast<float*>(xq + codes);
+    const int per_tile = p.gated ? 64 : 128;
+    long long chunks = (p.m + kCols - 1) / kCols;
+    if (p.offsets) chunks = chunks + p.n_exp < p.m ? chunks + p.n_exp : p.m;
+    const long long units = chunks * ((p.N + per_tile - 1) / per_tile);
+    FM_REQUIRE(units < (1ll << 30), kn, "%lld tiles are too many for one call", units);
+    // Rows that stay where they are can be read from there, half a group a box and every scale from a line of its own, which
+    // costs a step some 2 %; the kernel that orders them costs 2 to 3 us.  (77 rows, 40 steps: 24.6 us and 26.5; 2048 rows, 600
+    // steps: 373 and 363.)
+    const bool direct = !p.bucket_rows && (units + c.sm_count - 1) / c.sm_count * (p.K / 128) <= 200;
+    const long long rows = direct && p.offsets ? p.xrows : p.m;
+    const int8_t* x = p.ae;
+    Scales scales = {p.asc, p.K / 128, 1};
+    cudaError_t e;
+    if (!direct) {
+        const size_t codes = (size_t)p.m * p.K, bytes = codes + (size_t)p.m * (p.K / 128) * 4;
+        int8_t* ordered = static_cast<int8_t*>(engine_scratch(bytes));
+        FM_REQUIRE(ordered, kn, "the engine workspace cannot grow to %zu bytes here (inside a capture: raise FM_SCRATCH_MB)", bytes);
+        float* by_group = reinterpret_cast<float*>(ordered + codes);
+        size_t blocks = ((size_t)p.m * (p.K / 32) + 255) / 256;
+        if (blocks > (size_t)c.sm_count * 16) blocks = (size_t)c.sm_count * 16;
+        e = launch_kernel(order_codes_kernel, dim3((unsigned)blocks), dim3(256), 0, c.stream, pdl_enabled(), p, ordered, by_group);
+        if (e != cudaSuccess) return cuda_fail(kn, e);
+        const int rc = after_launch(kn);
+        if (rc != FM_OK) return rc;
+        x = ordered;
+        scales = {by_group, 1, p.m};
+    }
     CUtensorMap map_w;
-    RowMaps map_x;
-    const uint64_t wrows = (uint64_t)p.n_exp * p.N * (p.gated ? 2 : 1);
+    RowMaps map_x = {};
+    const uint64_t wrows = (uint64_t)p.n_exp * p.N * (p.gated ? 2 : 1), width = direct ? p.K / 2 : p.K;
     bool ok = wrows < 0x7fffffff && encode_bytes_box_map(&map_w, p.wq, wrows, (uint64_t)p.K / 2, 64, 64);
-    for (int b = 0; b < 4; b++) ok = ok && encode_bytes_box_map(&map_x.box[b], xq, (uint64_t)p.m, (uint64_t)p.K, 128, 128 >> b);
-    FM_REQUIRE(ok, kn, "the tensor maps of %llu rows of weights and %d rows of x were refused (K=%d)", (unsigned long long)wrows, p.m, p.K);
-    const size_t n = (size_t)p.m * (p.K / 32);
-    size_t eb = (n + 255) / 256;
-    if (eb > (size_t)c.sm_count * 16) eb = (size_t)c.sm_count * 16;
-    cudaError_t e = launch_kernel(order_codes_kernel, dim3((unsigned)eb), dim3(256), 0, c.stream, pdl_enabled(), p, xq, scales);
-    if (e != cudaSuccess) return cuda_fail(kn, e);
-    const int rc = after_launch(kn);
-    if (rc != FM_OK) return rc;
+    for (int b = 0; b < 4; b++) {
+        ok = ok && encode_bytes_box_map(&map_x.box[b], x, (uint64_t)rows, width, direct ? 64 : 128, 128 >> b);
+        if (direct) ok = ok && encode_bytes_box_map(&map_x.odd[b], p.ao, (uint64_t)rows, width, 64, 128 >> b);
+    }
+    FM_REQUIRE(ok, kn, "the tensor maps of %llu rows of weights and %lld rows of x were refused (K=%d)", (unsigned long long)wrows, rows, p.K);
     auto kern = p.gated ? tile_kernel<true> : tile_kernel<false>;
     const size_t smem = smem_bytes(p);
     if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return cuda_fail(kn, e);
-    const int rows = p.gated ? 64 : 128;
-    long long chunks = (p.m + kCols - 1) / kCols;
-    if (p.offsets) chunks = chunks + p.n_exp < p.m ? chunks + p.n_exp : p.m;
-    const long long units = chunks * ((p.N + rows - 1) / rows);
-    FM_REQUIRE(units < (1ll << 30), kn, "%lld tiles are too many for one call", units);
     const unsigned grid = (unsigned)(units < c.sm_count ? units : c.sm_count);
-    e = launch_kernel(kern, dim3(grid), dim3(kThreads), smem, c.stream, true, map_w, map_x, static_cast<const float*>(scales), p);
+    e = launch_kernel(kern, dim3(grid), dim3(kThreads), smem, c.stream, !direct || pdl_enabled(), map_w, map_x, scales, direct, p);
     return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
 }
 

@@ -194,5 +194,16 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
     return d;
 }
 
+// the same for rows of 64 bytes with the 64-byte swizzle (tile base 512-aligned): 8-row groups are 512 bytes apart
+__device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+    d |= (uint64_t)1 << 16;
+    d |= (uint64_t)((512 >> 4) & 0x3FFF) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)4 << 61;                       // layout type: 64-byte swizzle
+    return d;
+}
+
 }  // namespace tc
 }  // namespace fm

@@ -72,7 +72,7 @@ def test_dense_model_shapes(rt, m, n, k):
 # From here to the experts: enough rows and weights for the tensor-core tiles.  One group and odd numbers of groups, rows of
 # weights and of x that end inside a tile, more tiles than an SM (so that a CTA walks several).
 @pytest.mark.parametrize("m,n,k", [(300, 1000, 5120), (700, 1000, 1152), (4100, 129, 1152), (3000, 1000, 128), (129, 17408, 1152), (65, 17407, 1280),
-                                   (2049, 1300, 384)])
+                                   (2049, 1300, 384), (300, 1000, 25728)])
 def test_tiles_sizes(rt, m, n, k):
     _dense(rt, m, n, k)
 
