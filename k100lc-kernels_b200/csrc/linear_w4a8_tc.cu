@@ -19,8 +19,8 @@
 //   * eight warps, four for the even and four for the odd groups, drain the accumulators: C[m, n] = fmaf(float(I), ws * asc,
 //     C) in registers, then the epilogue.
 //
-// Measured (B200): 2048 x 17408 x 5120 with bias and gelu 361 us, 1.01 POP/s; the experts' gate and up projections of 1999
-// tokens, 8 of 64 experts of 1024 x 5120, 421 us.  What bounds it is the epilogue: a step of 128 x 128 sums takes its two
+// Measured (B200): 2048 x 17408 x 5120 with bias and gelu 361 to 368 us, 1.0 POP/s; the experts' gate and up projections of 1999
+// tokens, 8 of 64 experts of 1024 x 5120, 426 to 434 us; 77 gated rows of 6144 x 5120 24.6.  What bounds it is the epilogue: a step of 128 x 128 sums takes its two
 // sets 2000 clocks each (1000 a step; the MMAs 256), of which 1300 load, convert, scale and add and the rest waits for barriers
 // that are there and starts the next step; a tile ends with 5000 clocks in which nothing is multiplied.  Measured and
 // dropped: 16 columns loaded ahead of the 16 in work (396 us), 8 ahead of 8 (486 against 443 then), conversion by adding
