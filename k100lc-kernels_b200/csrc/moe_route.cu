@@ -95,7 +95,7 @@ __device__ __forceinline__ float resolution(const RouteParams& p, float most) {
 
 // ---- the decision in fp64: lane's experts lane * VPL + i, plain loops; taken for the few tokens that fp32 cannot decide
 template <int VPL>
-__device__ __noinline__ int decide64(const RouteParams& p, const float* __restrict__ xs, double* stage) {
+__device__ __forceinline__ int decide64(const RouteParams& p, const float* __restrict__ xs, double* stage) {
     const int lane = threadIdx.x & 31;
     double s[VPL];
     float x[VPL];
@@ -196,6 +196,45 @@ __device__ __forceinline__ uint32_t key_of(float v, int i) {
 }
 template <int VPL>
 __device__ __forceinline__ float value_of(uint32_t key) { return key_value(key & ~(uint32_t)(VPL - 1)); }
+
+// Whether an expert of the lane that is not chosen may have a larger key than `tie`, the first left out, from other inputs: by
+// the logits where they are the keys, by what fp32 can tell (the keys as route_token forms them) where there is a bias.  Equal
+// inputs on both sides of the cut are in the order of their index, but say nothing about the keys behind them.  (Experts of
+// groups that were dropped count as well: at worst the token is decided in fp64.)
+// id, value: the lane's choice and its key; m, z: maximum and sum of the softmax.
+template <int VPL, typename T>
+__device__ __forceinline__ bool hidden_by_tie(const RouteParams& p, size_t row, const float* xs, int id, float value, float m, float z) {
+    const int lane = threadIdx.x & 31, tie = __shfl_sync(0xffffffffu, id, p.topk);       // (topk < 32)
+    const float logit = logit_at(reinterpret_cast<const T*>(p.logits), row * p.n_exp + tie), bias = p.bias ? p.bias[tie] : 0.f;
+    value = __shfl_sync(0xffffffffu, value, p.topk);
+    uint32_t chosen = 0;
+    for (int j = 0; j < p.topk; j++) {
+        const int e = __shfl_sync(0xffffffffu, id, j);
+        if (e / VPL == lane) chosen |= 1u << (e % VPL);
+    }
+    const float r = 1.f / z;
+    bool hidden = false;
+#pragma unroll 1
+    for (int i = 0; i < VPL; i++) {
+        const float x = xs[i];
+        if (!(x > -INFINITY) || (chosen >> i & 1u)) continue;
+        if (!p.bias) {
+            hidden |= x > logit;
+            continue;
+        }
+        const float b = p.bias[lane * VPL + i], s = p.sigmoid ? rcp_approx(1.f + fast_exp(-x)) : x == m ? r : fast_exp(x - m) * r, key = s + b;
+        hidden |= !(x == logit && b == bias) && !(value - key > resolution<VPL>(p, fmaxf(fabsf(value), key > -INFINITY ? fabsf(key) : 0.f)));
+    }
+    return __any_sync(0xffffffffu, hidden);
+}
+
+// What the few tokens come to that fp32 may not decide: `near`, or else equal inputs on both sides of the cut and more keys close
+// behind them.
+template <int VPL, typename T>
+__device__ __noinline__ int decide_again(const RouteParams& p, size_t row, const float* xs, int id, float value, float m, float z, bool near, double* stage) {
+    if (!near && !hidden_by_tie<VPL, T>(p, row, xs, id, value, m, z)) return id;
+    return decide64<VPL>(p, xs, stage);
+}
 
 // Sorts the lane's keys, descending: Batcher's odd-even merge sort (1968).
 template <int VPL>
@@ -337,7 +376,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, size_t row, co
 #pragma unroll
     for (int i = 0; i < VPL; i++) key[i] = key_of<VPL>(!p.bias ? x[i] : x[i] > -INFINITY ? s[i] + bias[i] : -INFINITY, i);
     const bool check = p.bias || sizeof(T) == 4;                      // (16-bit logits themselves are exact keys)
-    bool near = false;
+    bool near = false, tie = false;
     float a = -INFINITY, b = -INFINITY;                               // the two best of the lane
     if (by_score) {
 #pragma unroll
@@ -388,19 +427,24 @@ __device__ __forceinline__ void route_token(const RouteParams& p, size_t row, co
     if (check) {
         const float v = value_of<VPL>(kept), prev = __shfl_up_sync(0xffffffffu, v, 1);
         const int before = __shfl_up_sync(0xffffffffu, id, 1);
-        bool close = lane > 0 && lane <= p.topk && id >= 0 && !(prev - v > resolution<VPL>(p, fmaxf(fabsf(v), fabsf(prev))));
+        const bool close = lane > 0 && lane <= p.topk && id >= 0 && !(prev - v > resolution<VPL>(p, fmaxf(fabsf(v), fabsf(prev))));
+        bool equal = false;
         if (close) {                                                  // equal inputs are equal keys: the order of the index is right
             const T* in = reinterpret_cast<const T*>(p.logits) + row * p.n_exp;
-            close = !(logit_at(in, id) == logit_at(in, before) && (!p.bias || p.bias[id] == p.bias[before]));
+            equal = logit_at(in, id) == logit_at(in, before) && (!p.bias || p.bias[id] == p.bias[before]);
         }
         // (the key after 32 choices has no lane to compare it in)
-        near = near || p.topk == 32 || __any_sync(0xffffffffu, close);
+        near = near || p.topk == 32 || __any_sync(0xffffffffu, close && !equal);
+        if (__any_sync(0xffffffffu, equal && lane == p.topk)) {       // is there more behind (`pick` took its own off the lists)
+            const float at = __shfl_sync(0xffffffffu, v, p.topk & 31), rest = value_of<VPL>(__reduce_max_sync(0xffffffffu, key[0]));
+            tie = !(at - rest > resolution<VPL>(p, fmaxf(fabsf(at), rest > -INFINITY ? fabsf(rest) : 0.f)));
+        }
     }
-    if (near) {
+    if (near || tie) {
         float copy[VPL];                                              // (an array whose address is taken lives in memory)
 #pragma unroll
         for (int i = 0; i < VPL; i++) copy[i] = x[i];
-        id = decide64<VPL>(p, copy, stage);
+        id = decide_again<VPL, T>(p, row, copy, id, value_of<VPL>(kept), m, z, near, stage);
     }
     if (lane >= p.topk) id = -1;
     // the weight of the lane's choice, from its logit

@@ -188,3 +188,61 @@ def test_route_and_plan_refuse(rt):
             with pytest.raises(RuntimeError, match="rejected"):
                 rt.launch("moe_plan_k", 1, 1, ok[:at] + [bad] + ok[at + 1:])
         rt.sync()
+
+
+def _tie_at_the_cut(rng, rows, n_exp, topk, kind):
+    """topk - 1 clear winners, `ties` equal inputs at the cut, and larger keys that fp32 does not tell from them, all at
+    random places -> logits, bias"""
+    x, bias = np.full((rows, n_exp), -5.0), None
+    if kind != "logits":
+        # the bias belongs to the expert: one order of the experts for all rows, the places of ties and larger keys differ
+        bias = np.full(n_exp, -1.0, np.float32)
+    order = rng.permutation(n_exp)
+    for r in range(rows):
+        winners, rest = order[: topk - 1], rng.permutation(order[topk - 1: topk + 15])
+        ties, more = rest[: 2 + r % 3], rest[4: 5 + r % 2]
+        if kind == "logits":
+            x[r, winners] = 2 + np.arange(topk - 1)
+            x[r, ties], x[r, more] = 1.0, np.nextafter(np.float32(1), np.float32(2))
+            continue
+        bias[winners], bias[order[topk - 1: topk + 15]] = 2 + np.arange(topk - 1), 0.25
+        x[r, winners], x[r, ties], x[r, more] = 5.0, *((20.0, 21.0) if kind == "sigmoid" else (-12.0, -11.0))
+    return x, bias
+
+
+@pytest.mark.parametrize("kind,dtype", [("logits", "f32"), ("sigmoid", "f32"), ("sigmoid", "bf16"), ("sigmoid", "f16"), ("softmax", "f32"), ("softmax", "bf16")])
+@pytest.mark.parametrize("topk", [1, 2, 8, 31])
+def test_route_larger_key_behind_a_tie_at_the_cut(rt, kind, dtype, topk):
+    rng = np.random.default_rng(topk)
+    for n_exp in (64, 256, 1000):
+        x, bias = _tie_at_the_cut(rng, 48, n_exp, topk, kind)
+        kw = dict(topk=topk, score="sigmoid" if kind == "sigmoid" else "softmax", bias=bias)
+        got, values = _run(rt, x, dtype, **kw)
+        _check(got, values, **kw)
+        # the same for one token, whose plan is made by the launch that routes
+        got, values = _run(rt, x[:1], dtype, **kw)
+        _check(got, values, **kw)
+
+
+def test_route_by_hand_behind_a_tie_at_the_cut(rt):
+    x = np.full((1, 256), -5, np.float32)
+    x[0, 0] = x[0, 8] = 1
+    x[0, 16] = np.nextafter(np.float32(1), np.float32(2))
+    assert _run(rt, x, topk=1)[0]["ids"].tolist() == [[16]]
+    x[0, 0] = x[0, 8] = 20
+    x[0, 16] = 21
+    assert _run(rt, x, topk=1, score="sigmoid", bias=np.zeros(256, np.float32))[0]["ids"].tolist() == [[16]]
+
+
+@pytest.mark.parametrize("n_exp,groups", [(32, 1), (60, 4), (256, 1), (256, 8)])
+@pytest.mark.parametrize("score,biased", [("softmax", False), ("softmax", True), ("sigmoid", True)])
+def test_route_of_few_levels(rt, n_exp, groups, score, biased):
+    """Logits of four levels, each moved by 0..2 steps of fp32: equal inputs and neighbours everywhere, at the cut too."""
+    rng = np.random.default_rng(n_exp + groups)
+    base = rng.integers(0, 4, size=(400, n_exp)) * 0.5 + 0.5
+    x = (base * (1 + rng.integers(0, 3, size=base.shape) * 2.0 ** -23)).astype(np.float32)
+    bias = np.full(n_exp, 0.5, np.float32) if biased else None
+    for topk in (1, 3, 8):
+        kw = dict(topk=topk, score=score, bias=bias, n_group=groups, topk_group=max(1, groups // 2), group_top=2 if groups > 1 else 1)
+        got, values = _run(rt, x, **kw)
+        _check(got, values, **kw)
