@@ -255,7 +255,7 @@ class MoEMLP:
             plan = self.router.forward_device(logits_dev, rows)
             h = self.ws.buffer(self.tag + ".h", pairs * self.gate_up.n * 4)
             d = self.ws.buffer(self.tag + ".d", pairs * self.dim * 4)
-            # a pair without a slot reads row 0 of the buckets with weight 0, which must be a number if there is no slot at all
+            # a pair without a slot names row 0 of the buckets: written even if no pair has a slot (the combine drops it, its weight is 0)
             rt.memset(d, 0, self.dim * 4)
             self.gate_up.forward_device(x_dev, plan, out_dev=h)
             self.down.forward_device(h, plan, gather=False, out_dev=d)

@@ -354,3 +354,26 @@ def test_products_refuse(rt):
             with pytest.raises(RuntimeError, match="rejected"):
                 rt.launch("moe_linear_w4a8_k", 1, 1, ok[:at] + [bad] + ok[at + 1:])
         rt.sync()
+
+
+@pytest.mark.parametrize("rows", [4, 260])
+def test_block_keeps_one_token_s_infinity_from_the_others(rt, rows):
+    """Token 0, which has the first slot of the buckets, overflows in the down product (values of 1e18 through weights of
+    60000; a quantiser in front of an infinity gives zeros); the others have choices without an expert."""
+    rng = np.random.default_rng(rows)
+    n_exp, dim, ffn = 5, 256, 128
+    x = rng.standard_normal((rows, dim)).astype(np.float32)
+    logits = rng.standard_normal((rows, n_exp)).astype(np.float32)
+    logits[0] = [9, 8, 0, 0, 0]
+    logits[1:, 1:] = -np.inf                               # one expert for two choices
+    wg, sg, _ = P.layer(rng, n_exp, 2 * ffn, dim)
+    wd, sd, _ = P.layer(rng, n_exp, dim, ffn)
+    with Bufs(rt) as b:
+        gate = ExpertLinear(rt, n_exp, ffn, dim, b.put(wg), b.put(sg), act="silu", gated=True)
+        down = ExpertLinear(rt, n_exp, dim, ffn, b.put(wd), b.put(np.full_like(sd, 60000)))
+        block = MoEMLP(rt, MoERouter(rt, n_exp, 2), gate, down)
+        want = block.forward(x, logits)
+        x[0] *= 1e18
+        got = block.forward(x, logits)
+    assert np.all(np.isfinite(want)) and not np.all(np.isfinite(got[0]))
+    assert np.array_equal(got[1:], want[1:])

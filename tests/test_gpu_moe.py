@@ -81,3 +81,29 @@ def test_moe_experts_over_quantized_layers(rt, path):
         experts = [Int4Linear(rt, out_dim, dim, p, s, path, ws, f"e{i}") for i, (p, s) in enumerate(packs[:2])]
         z = MoEExperts(rt, experts, 2, dim, out_dim, 1, ws).forward(x[:2], np.array([[-1], [7]]), np.ones((2, 1), np.float32))
     assert np.array_equal(z, np.zeros((2, out_dim), np.float32))
+
+
+def test_combine_skips_a_pair_of_weight_zero(rt):
+    """A choice without an expert has weight 0 and points to row 0 of the buckets, whatever that row holds: it adds nothing.
+    A weight that is not 0 brings an infinity or a NaN along as before."""
+    rng = np.random.default_rng(18)
+    rows, n_sel, dim = 6, 3, 132
+    bucket = rng.standard_normal((8, dim)).astype(np.float32)
+    bucket[0, ::2], bucket[0, 1::2] = np.inf, np.nan
+    weights = rng.random((rows, n_sel)).astype(np.float32)
+    base = rng.integers(1, 8, size=(rows, n_sel)).astype(np.uint32)
+    base[0, 1], weights[0, 1] = 0, 0
+    base[1, 0], weights[1, 0] = 0, -0.0
+    base[2], weights[2] = 0, 0                             # no expert at all
+    base[3, 2] = 0                                         # the row's own token
+    with Bufs(rt) as b:
+        y = b.zeros(rows * dim, np.float32, np.nan)
+        rt.launch("moe_combine_gather_k", rows, 64, [y, b.put(bucket), b.put(weights), b.put(base), n_sel, rows, dim])
+        got = b.get(y, rows * dim).reshape(rows, dim)
+    ref = np.zeros((rows, dim), np.float32)
+    for r in range(rows):
+        for e in range(n_sel):
+            if weights[r, e]:
+                ref[r] += weights[r, e] * bucket[base[r, e]]
+    assert np.array_equal(got, ref, equal_nan=True)
+    assert np.all(np.isfinite(got[[0, 1, 2, 4, 5]])) and not np.isfinite(got[3]).any()
