@@ -341,6 +341,19 @@ __device__ __forceinline__ void load_logits(const RouteParams& p, size_t row, fl
         if (!(x[i] > -INFINITY)) x[i] = -INFINITY;                    // NaN: never chosen
 }
 
+// Quotients of scores w some of which are below 2^-92 and may leave fp32's range (c: the lane's logit, -inf: no choice): all are
+// formed over exp(from), from being the largest chosen logit (of sigmoids: at most 0).  The sigmoid over it is
+// exp(c - from) / (1 + exp(c)) for c <= 0, and the second factor is 1 to fp32 below -64.
+__device__ __noinline__ float small_quotient(bool sigmoid, float c, float m, float w) {
+    const float most = key_value(__reduce_max_sync(0xffffffffu, ordered(c))), from = fminf(most, 0.f);
+    if (!sigmoid) w = m == INFINITY ? w : c == most ? 1.f : expf(c - most);
+    else if (from < 0.f) w = __fdiv_rn(expf(c - from), 1.f + expf(c));
+    else if (c < -64.f) w = expf(c);
+    if (!(c > -INFINITY)) w = 0.f;
+    const float sum = warp_sum(w);
+    return sum > 0.f ? __fdiv_rn(w, sum) : 0.f;
+}
+
 // One token: lane j < topk gets its j-th expert and weight.  Keys are formed and ordered in fp32; a token where two that
 // matter lie within the error of fp32 is decided again in fp64, so that the choice is that of the exact keys at fp32's cost.
 // bias: the lane's.
@@ -428,16 +441,15 @@ __device__ __forceinline__ void route_token(const RouteParams& p, size_t row, co
         const float v = value_of<VPL>(kept), prev = __shfl_up_sync(0xffffffffu, v, 1);
         const int before = __shfl_up_sync(0xffffffffu, id, 1);
         const bool close = lane > 0 && lane <= p.topk && id >= 0 && !(prev - v > resolution<VPL>(p, fmaxf(fabsf(v), fabsf(prev))));
-        bool equal = false;
-        if (close) {                                                  // equal inputs are equal keys: the order of the index is right
+        near = near || p.topk == 32;                                  // (the key after 32 choices has no lane to compare it in)
+        if (__any_sync(0xffffffffu, close)) {                         // equal inputs are equal keys: the order of the index is right
             const T* in = reinterpret_cast<const T*>(p.logits) + row * p.n_exp;
-            equal = logit_at(in, id) == logit_at(in, before) && (!p.bias || p.bias[id] == p.bias[before]);
-        }
-        // (the key after 32 choices has no lane to compare it in)
-        near = near || p.topk == 32 || __any_sync(0xffffffffu, close && !equal);
-        if (__any_sync(0xffffffffu, equal && lane == p.topk)) {       // is there more behind (`pick` took its own off the lists)
-            const float at = __shfl_sync(0xffffffffu, v, p.topk & 31), rest = value_of<VPL>(__reduce_max_sync(0xffffffffu, key[0]));
-            tie = !(at - rest > resolution<VPL>(p, fmaxf(fabsf(at), rest > -INFINITY ? fabsf(rest) : 0.f)));
+            const bool equal = close && logit_at(in, id) == logit_at(in, before) && (!p.bias || p.bias[id] == p.bias[before]);
+            near = near || __any_sync(0xffffffffu, close && !equal);
+            if (__any_sync(0xffffffffu, equal && lane == p.topk)) {   // is there more behind (`pick` took its own off the lists)
+                const float at = __shfl_sync(0xffffffffu, v, p.topk & 31), rest = value_of<VPL>(__reduce_max_sync(0xffffffffu, key[0]));
+                tie = !(at - rest > resolution<VPL>(p, fmaxf(fabsf(at), rest > -INFINITY ? fabsf(rest) : 0.f)));
+            }
         }
     }
     if (near || tie) {
@@ -448,16 +460,19 @@ __device__ __forceinline__ void route_token(const RouteParams& p, size_t row, co
     }
     if (lane >= p.topk) id = -1;
     // the weight of the lane's choice, from its logit
-    float w = 0.f;
+    float w = 0.f, c = -INFINITY;
     if (id >= 0) {
-        const float c = logit_at(reinterpret_cast<const T*>(p.logits), row * p.n_exp + id);
+        c = logit_at(reinterpret_cast<const T*>(p.logits), row * p.n_exp + id);
         if (p.sigmoid) w = __frcp_rn(1.f + expf(-c));
         else w = c == m ? 1.f : expf(c - m);
         if (!p.sigmoid && !p.renorm) w = __fdiv_rn(w, z);
     }
     if (p.renorm) {
-        const float sum = warp_sum(w);
-        w = sum > 0.f ? __fdiv_rn(w, sum) : 0.f;
+        // (a score below 2^-92 makes the sum -inf: it may be too small for fp32 where its quotient is not)
+        const float sum = warp_sum(id >= 0 && w < 0x1p-92f ? -INFINITY : w);
+        w = sum > 0.f ? __fdiv_rn(w, sum) : small_quotient(p.sigmoid, c, m, w);
+    } else if (p.sigmoid && c < -64.f) {
+        w = id >= 0 ? expf(c) : 0.f;                                  // (1 + exp(-c) ends with fp32's range)
     }
     weight = w * p.scale;
 }

@@ -246,3 +246,56 @@ def test_route_of_few_levels(rt, n_exp, groups, score, biased):
         kw = dict(topk=topk, score=score, bias=bias, n_group=groups, topk_group=max(1, groups // 2), group_top=2 if groups > 1 else 1)
         got, values = _run(rt, x, **kw)
         _check(got, values, **kw)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_route_weights_of_scores_that_underflow(rt, dtype):
+    """Chosen scores below fp32's range have an ordinary quotient.  (The logits differ by less than 64, so their difference
+    rounds by 2^-19 at most, which the weights' tolerance holds twice over.)"""
+    x = np.full((8, 16), -np.inf)
+    for r, v in enumerate(((-90, -91), (-100, -104), (-200, -201, -202.5), (-600, -600), (-16, -60), (-60, -90, -100), (-3, -63), (-63.5, -64.5, -88, -120))):
+        x[r, 3: 3 + len(v)] = v
+    kw = dict(topk=4, score="sigmoid", scale=2.5)
+    got, values = _run(rt, x, dtype, **kw)
+    _check(got, values, **kw)
+    assert np.allclose(got["w"][0, :2], [2.5 * 0.7310586, 2.5 * 0.2689414], rtol=1e-6)
+    # softmax: the bias takes the largest logit out of the choice
+    x = np.random.default_rng(1).standard_normal((40, 16)) * 3
+    x[:, 5] = np.linspace(60, 300, 40)
+    bias = np.linspace(0, 1, 16).astype(np.float32)
+    bias[5] = -np.inf
+    kw = dict(topk=4, bias=bias)
+    got, values = _run(rt, x, dtype, **kw)
+    _check(got, values, **kw)
+    # and so do the groups: one large expert alone against two of its size less something
+    x = np.random.default_rng(2).standard_normal((40, 16))
+    x[:, 0], x[:, 1:4] = 300, -np.inf
+    kw = dict(topk=2, n_group=4, topk_group=1, group_top=2, bias=np.where(np.arange(16) < 4, -2.0, 0).astype(np.float32))
+    got, values = _run(rt, x, dtype, **kw)
+    _check(got, values, **kw)
+
+
+def test_route_weights_at_the_type_s_lowest_value(rt):
+    """Equal scores have equal weights, however small; an infinite logit that the bias excludes leaves nothing to the others."""
+    x = np.full((2, 40), np.finfo(np.float32).min, np.float32)
+    x[1, 7] = 1.5
+    for score in ("softmax", "sigmoid"):
+        got, _ = _run(rt, x, topk=5, score=score)
+        assert got["ids"].tolist() == [[0, 1, 2, 3, 4], [7, 0, 1, 2, 3]]
+        assert np.allclose(got["w"], [[0.2] * 5, [1, 0, 0, 0, 0]], rtol=1e-6, atol=0)
+        assert got["offsets"][40] == 6
+    x = np.zeros((1, 8), np.float32)
+    x[0, 2] = np.inf
+    got, _ = _run(rt, x, topk=2, bias=np.where(np.arange(8) == 2, -5, 0).astype(np.float32))
+    assert got["ids"].tolist() == [[0, 1]] and not got["w"].any()
+
+
+def test_route_sigmoid_weights_below_the_normal_numbers(rt):
+    """Without renormalisation the weight is the score itself, a subnormal number between logits of -87 and -103: within two
+    steps of 2^-149 of its value, and a pair with a slot."""
+    x = np.array([[-80, -87, -88, -89, -95, -100, -102, -110]], np.float32)
+    got, _ = _run(rt, x, topk=8, score="sigmoid", renorm=False)
+    want = 1 / (1 + np.exp(-x.astype(np.float64)))
+    assert got["ids"].tolist() == [[0, 1, 2, 3, 4, 5, 6, 7]]
+    assert np.all(np.abs(got["w"] - want) <= P.ROUTE_REL * want + 3 * 2.0 ** -149)
+    assert got["offsets"][8] == 7                          # the score at -110 is 0 in fp32
