@@ -377,3 +377,32 @@ def test_block_keeps_one_token_s_infinity_from_the_others(rt, rows):
         got = block.forward(x, logits)
     assert np.all(np.isfinite(want)) and not np.all(np.isfinite(got[0]))
     assert np.array_equal(got[1:], want[1:])
+
+
+@pytest.mark.parametrize("rows,n,k", [(16, 40, 256), (5, 100, 1152), (16, 700, 1024), (3000, 300, 1152)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_experts_slot_without_a_row_of_x(rt, rows, n, k, gated):
+    """A row index outside of x stands for a row of zeros, with few rows and on tiles."""
+    rng = np.random.default_rng(rows + n)
+    wq, ws, w = P.layer(rng, 2, n * (2 if gated else 1), k)
+    cd, q = P.codes(rng, rows, k)
+    bias = rng.standard_normal((2, w.shape[1])).astype(np.float32)
+    bucket = rng.integers(0, rows, rows).astype(np.int32)
+    for i, bad in enumerate((-1, rows, 2 ** 31 - 1, -2 ** 31)):
+        bucket[i::5] = bad
+    offsets = np.array([0, rows // 3, rows], np.int32)
+    with Bufs(rt) as b:
+        lin = ExpertLinear(rt, 2, n, k, b.put(wq), b.put(ws), bias=bias, act="silu", gated=gated)
+        plan = MoEPlan(rows=rows, topk=1, n_exp=2, ids=0, weights=0, bucket_rows=b.put(bucket), base=0, offsets=b.put(offsets))
+        out = b.zeros(rows * n, np.float32, -777.0)
+        lin.forward_codes_device([b.put(c) for c in cd], plan, out_dev=out)
+        got = b.get(out, rows * n).reshape(rows, n)
+        assert rt.gemm_status() == 0
+        lin.ws.free()
+    known = (bucket >= 0) & (bucket < rows)
+    at = np.where(known, bucket, 0)
+    q, asc = np.where(known[:, None], q[at], 0), np.where(known[:, None], cd[2][at], 0).astype(np.float32)
+    for e in range(2):
+        lo, hi = offsets[e], offsets[e + 1]
+        want, bound = P.epilogue(*P.product(w[e], ws[e], q[lo:hi], asc[lo:hi]), "silu", gated, bias[e], None)
+        _within(got[lo:hi], want, bound)
