@@ -406,3 +406,34 @@ def test_experts_slot_without_a_row_of_x(rt, rows, n, k, gated):
         lo, hi = offsets[e], offsets[e + 1]
         want, bound = P.epilogue(*P.product(w[e], ws[e], q[lo:hi], asc[lo:hi]), "silu", gated, bias[e], None)
         _within(got[lo:hi], want, bound)
+
+
+@pytest.mark.parametrize("m", [3, 3000])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_activations_in_their_tails(rt, m, act):
+    """Codes of zero leave the bias, here from -30 to 30, as the activation's argument v.
+    2^-20 |v| everywhere: the erf formula is within 1.5e-7, the roundings of its reciprocal (times a slope of 3.5 at most),
+    five steps and exp within 1.3e-6, half of both times |v|; the logistic forms have a reciprocal, an exp whose argument's
+    error is damped by s (1 - s) |t| < 1/4, and three products.
+    Left of 0 the result is a small number of its own: v / 2 times erfc, whose formula is within 3.9 % of it up to
+    |v| = 13.3 (compared in 64 bits), or v / (1 + exp(t)) with t within 2^-21 of its value, t <= 88.  Behind that
+    it is below 2^-126 |v|, where the reciprocal and exp give 0."""
+    from scipy.special import erfc
+    n, k = 600, 1152
+    v = np.linspace(-30, 30, n).astype(np.float32)
+    wq, ws, _ = P.layer(np.random.default_rng(1), 1, n, k)
+    zero = np.zeros((m, k // 2), np.int8)
+    with Bufs(rt) as b:
+        lin = FusedLinear(rt, n, k, b.put(wq), b.put(ws), bias=v, act=act)
+        out = b.zeros(m * n)
+        lin.forward_codes_device([b.put(zero), b.put(zero), b.zeros(m * k // 128), b.zeros(m * k // 128, np.int32)], m, out_dev=out)
+        got = b.get(out, m * n).reshape(m, n)
+        lin.ws.free()
+    x = v.astype(np.float64)
+    with np.errstate(over="ignore"):
+        want = {"gelu": x / 2 * erfc(-x / np.sqrt(2)), "silu": x / (1 + np.exp(-x)),
+                "gelu_tanh": x / (1 + np.exp(-2 * np.sqrt(2 / np.pi) * (x + 0.044715 * x ** 3)))}[act]
+    assert np.all(np.abs(got - want) <= 2.0 ** -20 * np.abs(v))
+    left = v < 0
+    assert np.all(np.abs(got - want)[:, left] <= (0.05 * np.abs(want) + 2.0 ** -125 * np.abs(v))[left])
+    assert np.all(got == got[0])
