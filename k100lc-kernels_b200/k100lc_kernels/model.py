@@ -49,21 +49,30 @@ def div_magic(d: int, max_i: int) -> int:
 
 class Workspace:
     """Device buffers re-used by key: ``buffer(key, nbytes)`` returns the same block for
-    the same key and re-allocates only when it has to grow."""
+    the same key and re-allocates only when it has to grow.  While a captured graph is alive,
+    whose kernels may hold the outgrown block's address, that block is kept."""
 
     def __init__(self, rt: Runtime):
         self.rt = rt
         self._bufs: dict[str, tuple[int, int]] = {}
+        self._outgrown: list[int] = []
 
     def buffer(self, key: str, nbytes: int) -> int:
         have = self._bufs.get(key)
         if have and have[1] >= nbytes:
             return have[0]
         if have:
-            self.rt.free(have[0])
+            del self._bufs[key]
+            self._outgrown.append(have[0])
+            if not getattr(self.rt, "graphs_alive", False):
+                self._free_outgrown()
         p = self.rt.alloc(int(nbytes))
         self._bufs[key] = (p, int(nbytes))
         return p
+
+    def _free_outgrown(self) -> None:
+        while self._outgrown:
+            self.rt.free(self._outgrown.pop())
 
     def upload(self, key: str, data) -> int:
         n = len(data) if isinstance(data, (bytes, bytearray, memoryview)) else data.nbytes
@@ -78,6 +87,7 @@ class Workspace:
         for p, _n in self._bufs.values():
             self.rt.free(p)
         self._bufs.clear()
+        self._free_outgrown()
 
     def __enter__(self):
         return self

@@ -214,6 +214,7 @@ class Runtime:
         self._names_by_id: dict[int, str] = {}
         self._pending: list | None = None
         self._argv = (ctypes.c_uint64 * 32)()
+        self._graphs: set = set()                # captured graphs that are alive (None: the one being captured)
 
     # ---- helpers ---------------------------------------------------------------
     def _name(self, kernel: str) -> bytes:
@@ -427,11 +428,14 @@ class Runtime:
     def graph_begin(self) -> None:
         if self._lib.fm_graph_begin() != 0:
             self._fail("fm_graph_begin")
+        self._graphs.add(None)
 
     def graph_end(self) -> int:
         g = self._lib.fm_graph_end()
+        self._graphs.discard(None)
         if g < 0:
             self._fail("fm_graph_end")
+        self._graphs.add(g)
         return g
 
     def graph_launch(self, graph: int) -> None:
@@ -440,6 +444,12 @@ class Runtime:
 
     def graph_free(self, graph: int) -> None:
         self._lib.fm_graph_free(graph)
+        self._graphs.discard(graph)
+
+    @property
+    def graphs_alive(self) -> bool:
+        """Whether a graph of ``graph_begin`` / ``graph_end`` is being captured or has not been freed."""
+        return bool(self._graphs)
 
     def stream_table(self, layers, rows: int, k: int, row_base: int = 0, dev: int | None = None) -> int:
         """Validated device table for ``w4a8_decode_stream``: ``layers`` is a list of

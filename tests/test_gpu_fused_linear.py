@@ -437,3 +437,26 @@ def test_activations_in_their_tails(rt, m, act):
     left = v < 0
     assert np.all(np.abs(got - want)[:, left] <= (0.05 * np.abs(want) + 2.0 ** -125 * np.abs(v))[left])
     assert np.all(got == got[0])
+
+
+def test_block_in_a_graph_outlives_a_larger_call(rt):
+    """A graph of few rows is replayed after a call of many, for which every buffer of the block grew."""
+    rng = np.random.default_rng(7)
+    dim, few, many = 256, 5, 700
+    with Bufs(rt) as b:
+        block = _block(rt, b, rng, 5, 2, dim, 128)
+        px, pl, py = b.zeros(few * dim), b.zeros(few * 5), b.zeros(few * dim)
+        block.forward_device(px, pl, few, out_dev=py, sync=True)
+        rt.graph_begin()
+        block.forward_device(px, pl, few, out_dev=py)
+        graph = rt.graph_end()
+        for _ in range(2):
+            x, logits = rng.standard_normal((few, dim)).astype(np.float32), rng.standard_normal((few, 5)).astype(np.float32)
+            want = block.forward(x, logits)
+            block.forward(rng.standard_normal((many, dim)).astype(np.float32), rng.standard_normal((many, 5)).astype(np.float32))
+            many *= 2
+            rt.upload(px, x)
+            rt.upload(pl, logits)
+            rt.graph_launch(graph)
+            assert np.array_equal(b.get(py, few * dim).reshape(few, dim), want)
+        rt.graph_free(graph)
