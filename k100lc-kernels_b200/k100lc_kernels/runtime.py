@@ -128,9 +128,25 @@ def load_library(path=None) -> ctypes.CDLL:
     return lib
 
 
+class _InOrder:
+    """The library inside a batch scope: a call that works on the device comes after the launches recorded in front of it."""
+
+    _ASIDE = {"fm_alloc", "fm_host_alloc", "fm_kernel_id", "fm_kernel_name", "fm_has_kernel", "fm_device_attr", "fm_last_error"}
+
+    def __init__(self, rt: "Runtime", lib):
+        self._rt, self._lib = rt, lib
+
+    def __getattr__(self, name):
+        if name not in self._ASIDE and self._rt._pending:
+            calls, self._rt._pending = self._rt._pending, []
+            LaunchPlan(self._rt, calls).run()
+        return getattr(self._lib, name)
+
+
 class _BatchScope:
     """``with rt.batch():`` — launches inside are recorded and handed to the engine as
-    one plan on exit (reference runtime.py:30-47, 267-298)."""
+    one plan on exit (reference runtime.py:30-47, 267-298), or before the next call of another
+    kind (``launch2d``, an upload, a synchronisation), so that the order is that of the calls."""
 
     def __init__(self, rt: "Runtime"):
         self._rt = rt
@@ -139,10 +155,12 @@ class _BatchScope:
         if self._rt._pending is not None:
             raise RuntimeError("batch() scopes do not nest")
         self._rt._pending = []
+        self._rt._lib = _InOrder(self._rt, self._rt._lib)
         return self
 
     def __exit__(self, exc_type, exc, tb):
         calls, self._rt._pending = self._rt._pending, None
+        self._rt._lib = self._rt._lib._lib
         if exc_type is None and calls:
             LaunchPlan(self._rt, calls).run()
         return False

@@ -460,3 +460,30 @@ def test_block_in_a_graph_outlives_a_larger_call(rt):
             rt.graph_launch(graph)
             assert np.array_equal(b.get(py, few * dim).reshape(few, dim), want)
         rt.graph_free(graph)
+
+
+@pytest.mark.parametrize("rows", [6, 40])
+def test_block_in_a_batch_scope(rt, rows):
+    """Two blocks behind each other, and a layer on their output: the quantisers between the recorded launches take their
+    turn."""
+    rng = np.random.default_rng(rows)
+    dim = 256
+    x, logits = rng.standard_normal((rows, dim)).astype(np.float32), rng.standard_normal((rows, 5)).astype(np.float32)
+    with Bufs(rt) as b:
+        block = _block(rt, b, rng, 5, 2, dim, 128)
+        wq, ws, _ = P.layer(rng, 1, dim, dim)
+        lin = FusedLinear(rt, dim, dim, b.put(wq), b.put(ws), act="gelu")
+        px, pl, pa, pb, pc = b.put(x), b.put(logits), b.zeros(rows * dim), b.zeros(rows * dim), b.zeros(rows * dim)
+
+        def run():
+            block.forward_device(px, pl, rows, out_dev=pa)
+            block.forward_device(pa, pl, rows, out_dev=pb)
+            return lin.forward_device(pb, rows, out_dev=pc)
+
+        run()
+        want = b.get(pc, rows * dim)
+        for p in (pa, pb, pc):
+            rt.memset(p, 0, rows * dim * 4)
+        with rt.batch():
+            run()
+        assert np.any(want) and np.array_equal(b.get(pc, rows * dim), want)
