@@ -239,12 +239,15 @@ int run_rows(const char* kn, const LaunchCtx& c, const Params& p) {
     return e == cudaSuccess ? after_launch(kn) : cuda_fail(kn, e);
 }
 
-// Rows or tiles, whichever promises to be done first.  The rows kernel reads the weights of a bucket once for every 8 rows, at
-// 5.6 MB a microsecond and more; a tile takes 0.35 us for a 128-group, one wave of tiles after the other, 2.5 us later than
-// the rows kernel starts.  (Buckets as if all experts were equally popular, half a piece added for the rest of each.)
-// Measured, rows against tiles: 17408 x 5120 at 16 rows 19.0 and 22.3 us, at 17 rows 27.3 and 23.1; 5120 x 17408 at 32 rows 53.8
-// and 54.6; 2048 x 2048 at 48 rows 8.1 and 13.8; 8 of 64 gated experts of 1024 x 5120 at 72 tokens 94 and 109, at 128 142
-// and 114.
+// Rows or tiles, whichever promises to be done first.  The rows kernel passes over the weights of a bucket once for every 8 rows:
+// counted at 5.7 MB a microsecond, measured 3.3 (5120 x 17408, whose few units leave warps idle: 32 to 56 rows all take 54 us) to
+// 5.8 (the experts below).  A tile is counted at 0.35 us for a 128-group, one wave of tiles after the other, 2.5 us later than the
+// rows kernel starts, measured 0.35 to 0.42.  (Buckets as if all experts were equally popular, half a piece added for the rest of
+// each.)
+// Measured, rows against tiles: 17408 x 5120 at 16 rows 19.0 and 22.3 us, at 17 rows 27.3 and 23.1; 5120 x 17408 at 32 rows 53.4
+// and 53.3, at 40 53.8 and 59.4, at 48 53.8 and 59.2 (the last that goes to the rows kernel), at 56 54.0 and 59.5, at 64 73.8 and
+// 59.5; 5120 x 5120 at 48 rows 20.5 and 20.8, at 64 25.4 and 22.6; 2048 x 2048 at 48 rows 8.2 and 12.4, at 128 12.3 and 14.5; 8 of
+// 64 gated experts of 1024 x 5120 at 72 tokens 94 and 109, at 128 142 and 114.
 bool rows_first(const LaunchCtx& c, const Params& p) {
     const long long used = !p.offsets ? 1 : p.n_exp < p.m ? p.n_exp : p.m, rows = p.gated ? 64 : 128;
     auto pieces = [&](int of) {
