@@ -22,7 +22,7 @@
 // that group of the current one, so that 4 KB a warp are on their way at any time, across the ends of its units too.  Where
 // there are fewer units than warps the K dimension is split over the warps of a team and their partial sums meet in shared
 // memory.  Measured (B200, cold weights): one row of 17408 x 5120 12.3 us (11.0 in a graph, 4.2 TB/s; 8 rows 11.9), five rows of
-// 5120 x 17408 18.1 us (16.0), 33 tokens through 8 of 64 experts of 5120 x 1024 38.5 us (4.6 TB/s, 0.70 of a copy's rate): what is left
+// 5120 x 17408 18.3 us (16.0), 33 tokens through 8 of 64 experts of 5120 x 1024 35 to 38 us (4.6 to 5 TB/s, 0.70 to 0.76 of a copy's rate): what is left
 // is the time from a launch to the first weights and the last unit's tail.
 #include <cuda_fp16.h>
 

@@ -22,8 +22,8 @@
 // A warp takes a token and holds its experts in registers, neighbours to a lane, so that a group is a run of lanes: scores, a
 // sort of the lane's keys, the groups' worths by shuffles, and topk rounds of a warp-wide maximum over the lanes' best.
 // Measured (B200): one token of 128 experts 7.2 us (a launch), 48 of 256 in groups 11.9, 3001 of 60 14.3, 16384 of 256 (bf16,
-// sigmoid, bias, 4 of 8 groups, 8 choices) 47 us, 222 GB/s.  Bound by instructions: 1100 of a warp for a token, issued in 59 % of
-// the cycles; the bytes would take 1.6 us.
+// sigmoid, bias, 4 of 8 groups, 8 choices) 48 us, 219 GB/s.  Bound by instructions: 1140 of a warp for a token, issued in 58 % of
+// the cycles; the bytes would take 1.6 us.  (16384 tokens of 256 equal logits, f32, 39 us: see decide_again.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -355,7 +355,7 @@ __device__ __noinline__ float small_quotient(bool sigmoid, float c, float m, flo
 }
 
 // One token: lane j < topk gets its j-th expert and weight.  Keys are formed and ordered in fp32; a token where two that
-// matter lie within the error of fp32 is decided again in fp64, so that the choice is that of the exact keys at fp32's cost.
+// matter lie within the error of fp32 is decided again in fp64, so that the choice is that of the keys in fp64 at fp32's cost.
 // bias: the lane's.
 template <int VPL, typename T>
 __device__ __forceinline__ void route_token(const RouteParams& p, size_t row, const float (&bias)[VPL], double* stage, int& id, float& weight) {

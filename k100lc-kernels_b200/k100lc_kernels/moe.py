@@ -206,8 +206,8 @@ class ExpertLinear(_Product):
     def forward_codes_device(self, codes, plan: MoEPlan, gather: bool = True, out_dev: int | None = None,
                              sync: bool = False) -> int:
         """-> ``[plan.rows * plan.topk, n]`` f32 in bucket order.  ``gather``: the codes are those of the tokens and a
-        slot takes its token's row; otherwise they are in bucket order already.  Rows behind the last bucket are left
-        as they were."""
+        slot takes its token's row (a row index outside of them: a row of zeros); otherwise they are in bucket order
+        already.  Rows behind the last bucket are left as they were."""
         if plan.n_exp != self.n_exp:
             raise ValueError(f"the plan is for {plan.n_exp} experts, the layer has {self.n_exp}")
         pairs = plan.rows * plan.topk
